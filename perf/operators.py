@@ -219,8 +219,10 @@ def _inputs(case, seed):
         t["positions"] = torch.randint(0, case["far"], (case["axes"], n), generator=gen, device=dev).to(torch.int32)
         i = np.arange(case["rot"] // 2)
         t["freqs"] = torch.from_numpy((1e6 ** (-2.0 * i / case["rot"])).astype(np.float32)).to(dev)
-        places = t["k_cache"].shape[0] * case["page"]
-        slots = rnd.permutation(places)[:n].astype(np.int64)
+        # consecutive places of pages in any order, from somewhere in the first of them
+        pages = rnd.permutation(t["k_cache"].shape[0])
+        slots = (pages[:, None].astype(np.int64) * case["page"] + np.arange(case["page"])).reshape(-1)
+        slots = slots[rnd.randint(0, 2 * case["page"]):][:n]
         slots[rnd.randint(0, n, case["skip"] if n > 1 else 0)] = -1
         t["slots"] = _ints(slots, dev)
         t["q_out"] = torch.zeros((n, hq * d), device=dev)
