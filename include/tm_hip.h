@@ -4,8 +4,9 @@
  *
  * This is the HIP counterpart of the reference's Metal ABI
  * (native/metal/tm_metal.h): the same conventions, restricted to what the
- * Q8_0 decode GEMV / prefill GEMM / embedding-row path needs. Every entry
- * point names the reference declaration it stands in for.
+ * Q8_0 decode GEMV / prefill GEMM / embedding-row path needs, and the operators
+ * between a step's products. Every entry point that stands in for a reference
+ * declaration names it.
  *
  * Conventions (native/metal/tm_metal.h:1-18, :32-40):
  *   - One context owns one device, one HIP stream and the loaded kernels.
@@ -91,6 +92,13 @@ void tm_hip_buffer_free(tm_hip_ctx *ctx, tm_hip_buffer *buffer);
 
 /* Length in bytes, 0 for an invalid handle (native/metal/tm_metal.h:73). */
 size_t tm_hip_buffer_len(const tm_hip_ctx *ctx, const tm_hip_buffer *buffer);
+
+/* The buffer's device address, for programs that read or fill it with kernels of
+ * their own on another stream; tm_hip_fence orders the context's work before
+ * that, the caller's own synchronization after it. Valid until buffer_free; NULL
+ * for an invalid handle, a private buffer or sealed weights
+ * (native/metal/tm_metal.h:68-70). */
+void *tm_hip_buffer_contents(const tm_hip_ctx *ctx, const tm_hip_buffer *buffer);
 
 /* Zero `len` bytes at byte offset `off` on the device, ordered with the
  * context's other work (native/metal/tm_metal.h:78-79). */
@@ -294,6 +302,138 @@ int tm_hip_f16_gemm(tm_hip_ctx *ctx, tm_hip_buffer *w, tm_hip_buffer *x, tm_hip_
  * (native/metal/tm_metal.h:155-157). */
 int tm_hip_f16_row_f32(tm_hip_ctx *ctx, tm_hip_buffer *w, tm_hip_buffer *out, uint32_t row,
                        uint32_t cols, uint32_t out_off, char *err, size_t err_cap);
+
+/* ---- the operators between a step's products: positions, key-value cache,
+ * attention, logits ---------------------------------------------------------
+ * All take f32 activations, run on the context's stream like every operator
+ * here, are usable inside a dispatch group and in recorded steps, and read what
+ * changes from token to token (positions, slots, page tables, lengths,
+ * histories) from device buffers: a recorded step is replayed for the next
+ * token after those have been written. Ids and lengths are uint32_t. A buffer
+ * named as an output must not be named as anything else in the same call,
+ * unless the entry point says so. Sealed weight buffers are refused. */
+
+/* A paged key-value cache: two buffers of `pages` pages each,
+ *   k  [page][kv_head][place][channel]
+ *   v  [page][kv_head][channel][place]
+ * of F16 (type_id 1) or F32 (type_id 0) elements: a token's key is contiguous,
+ * and so are a value channel's places, which is how each of the two products
+ * of the attention reads its operand. page_tokens (places per page) is a power
+ * of two from 16 to 256, head_dim a multiple of 8 up to 256. A slot is
+ * page * page_tokens + place. The struct is a description, copied by the call. */
+typedef struct tm_hip_kv_cache {
+    tm_hip_buffer *k, *v;
+    uint32_t type_id, pages, page_tokens, kv_heads, head_dim;
+} tm_hip_kv_cache;
+
+/* Rotary positions over the first `rot_dim` channels of a head (even). Pair i of
+ * rot_dim / 2 is channels (i, i + rot_dim / 2), or (2i, 2i + 1) where `adjacent`
+ * is not 0; it turns by positions[axis(i)][token] * freqs[i] radians, the
+ * product and its reduction to one turn taken in 64 bits. `axes` is 1..4 and
+ * sections[a] the number of pairs that axis a turns (they add up to
+ * rot_dim / 2): axis 0 has the first sections[0] pairs and so on, or, where
+ * `interleaved` is not 0, the axes take pairs in turn until their sections are
+ * used up. */
+typedef struct tm_hip_rope {
+    tm_hip_buffer *freqs; /* f32 [rot_dim / 2] */
+    uint32_t rot_dim, axes, sections[4], interleaved, adjacent;
+} tm_hip_rope;
+
+/* For `tokens` rows: q_out = q turned, and the turned k and the plain v rounded
+ * once to the cache's type and stored at slots[token] (a slot outside the cache
+ * stores nothing; of several rows that name one slot the last is stored). Row t
+ * of q starts at element q_off + t * q_stride and holds q_heads * head_dim
+ * values (k, v: kv_heads * head_dim); a stride of 0 means packed rows.
+ * positions is [axes][tokens]. q, k and v may lie in one buffer (the rows of a
+ * fused projection), and q_out may be q in place (same offset and stride);
+ * any other overlap of q_out with q, k or v is refused. tokens is at most
+ * TM_HIP_KV_MAX_TOKENS. */
+#define TM_HIP_KV_MAX_TOKENS (1u << 20)
+#define TM_HIP_KV_MAX_SEQS 32768u
+#define TM_HIP_KV_MAX_HEADS 1024u
+int tm_hip_rope_store_f32(tm_hip_ctx *ctx, const tm_hip_rope *rope, const tm_hip_kv_cache *cache,
+                          tm_hip_buffer *q, tm_hip_buffer *k, tm_hip_buffer *v,
+                          tm_hip_buffer *q_out, tm_hip_buffer *positions, tm_hip_buffer *slots,
+                          uint32_t tokens, uint32_t q_heads, uint32_t q_off, uint32_t k_off,
+                          uint32_t v_off, uint32_t out_off, uint32_t q_stride, uint32_t k_stride,
+                          uint32_t v_stride, uint32_t out_stride, char *err, size_t err_cap);
+
+/* What a query at position p of a sequence of `len` cached tokens sees, and how
+ * its scores are made. With head h reading key-value head h / (q_heads /
+ * kv_heads), position j of the sequence is visible where
+ *     max(first, p - window + 1) <= j < min(len, max(p + 1, prefix))
+ * (window 0: no window) and its score is
+ *     x = scale * dot(q, k_j);  softcap > 0: x = softcap * tanh(x / softcap);
+ *     slopes: x -= slopes[h] * |p - j|
+ * out = sum_j softmax(x)_j * v_j. Where nothing is visible, or every visible
+ * score is -infinity, out is zero. What is cached at positions a query does not
+ * see has no influence on it, infinities and NaN included. Scores, softmax
+ * statistics and sums are f32; over F16 pages q and the softmax weights enter the
+ * matrix products as the sum of two f16 numbers (22 bits), not rounded to one.
+ * slopes (f32 [q_heads]), first (u32, one per query row: where its document
+ * begins) and prefix (u32, one per sequence: leading positions that every query
+ * of the sequence sees) may be NULL. */
+typedef struct tm_hip_attn {
+    float scale, softcap;
+    uint32_t window;
+    tm_hip_buffer *slopes, *first, *prefix;
+} tm_hip_attn;
+
+/* One query per sequence, at the sequence's last cached position (p = len - 1):
+ * out[s] = attention of q[s] over the first lens[s] positions of sequence s.
+ * Position j lies in page table[s * table_stride + j / page_tokens] at place
+ * j % page_tokens; positions in pages that are not in the cache are not
+ * visible, and lens is cut at table_stride * page_tokens (which is at most
+ * 2^31 - 1). Rows of q and out are q_heads * head_dim values from q_off, out_off,
+ * strides of 0 mean packed. q_heads is a multiple of kv_heads. A long sequence is
+ * split over workgroups and joined in the same launch, in the order of
+ * positions: the same call gives the same bits. */
+int tm_hip_attn_decode_f32(tm_hip_ctx *ctx, const tm_hip_attn *attn, const tm_hip_kv_cache *cache,
+                           tm_hip_buffer *q, tm_hip_buffer *table, tm_hip_buffer *lens,
+                           tm_hip_buffer *out, uint32_t seqs, uint32_t q_heads,
+                           uint32_t table_stride, uint32_t q_off, uint32_t out_off,
+                           uint32_t q_stride, uint32_t out_stride, char *err, size_t err_cap);
+
+/* A ragged batch of query rows: rows starts[s] .. starts[s + 1] (of `tokens`;
+ * starts has seqs + 1 entries and ascends) are the last positions of sequence s,
+ * whose lens[s] cached tokens include them (tm_hip_rope_store_f32 has stored
+ * them). Rows in no sequence (behind starts[seqs], or of a sequence whose
+ * bounds do not ascend within `tokens`) keep what out held. Otherwise as
+ * tm_hip_attn_decode_f32; attn->first has an entry per row. */
+int tm_hip_attn_prefill_f32(tm_hip_ctx *ctx, const tm_hip_attn *attn, const tm_hip_kv_cache *cache,
+                            tm_hip_buffer *q, tm_hip_buffer *table, tm_hip_buffer *lens,
+                            tm_hip_buffer *starts, tm_hip_buffer *out, uint32_t tokens,
+                            uint32_t seqs, uint32_t q_heads, uint32_t table_stride, uint32_t q_off,
+                            uint32_t out_off, uint32_t q_stride, uint32_t out_stride, char *err,
+                            size_t err_cap);
+
+/* What is done to a row of logits before a token is picked from it. With c the
+ * number of times id is among the first history_len[row] entries of the row's
+ * history (u32 [rows][history_stride]; ids outside the vocabulary count for
+ * nothing, lengths are cut at the stride):
+ *     c > 0:   x = x > 0 ? x / penalties[row][0] : x * penalties[row][0];
+ *              x -= penalties[row][1] + penalties[row][2] * c
+ *     biases:  x += bias_values of the last of the row's first bias_len[row]
+ *              entries whose bias_ids is id
+ *     allowed: x = -infinity unless bit id % 32 of word
+ *              row * allowed_stride + id / 32 is set
+ * history, history_len and penalties (f32 [rows][3]: repetition, presence,
+ * frequency) come together or are all NULL, and so do bias_ids, bias_values
+ * ([rows][bias_stride]) and bias_len; allowed may be NULL. */
+typedef struct tm_hip_logits_adjust {
+    tm_hip_buffer *history, *history_len, *penalties;
+    tm_hip_buffer *bias_ids, *bias_values, *bias_len;
+    tm_hip_buffer *allowed;
+    uint32_t history_stride, bias_stride, allowed_stride;
+} tm_hip_logits_adjust;
+
+/* out[row][id] = adjusted logits[row][id] for rows x vocab values from element
+ * x_off of logits and y_off of out; out may be logits in place (same offset).
+ * rows is at most TM_HIP_KV_MAX_SEQS. tm_hip_argmax_f32 picks from the result. */
+int tm_hip_logits_adjust_f32(tm_hip_ctx *ctx, const tm_hip_logits_adjust *adjust,
+                             tm_hip_buffer *logits, tm_hip_buffer *out, uint32_t rows,
+                             uint32_t vocab, uint32_t x_off, uint32_t y_off, char *err,
+                             size_t err_cap);
 
 /* ---- additions with no Metal counterpart ---- */
 

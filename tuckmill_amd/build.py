@@ -22,9 +22,10 @@ DEVICE_FLAGS = [
 ]
 
 
-# The library is two translation units: the host logic (tm_hip.cpp: no device
-# code, seconds to compile) and the kernels with their launchers (tm_launch.cpp).
-SOURCES = ("tm_hip.cpp", "tm_launch.cpp")
+# The library is three translation units: the host logic (tm_hip.cpp: no device
+# code, seconds to compile), the products' kernels with their launchers
+# (tm_launch.cpp) and those of the operators between products (tm_kv.cpp).
+SOURCES = ("tm_hip.cpp", "tm_launch.cpp", "tm_kv.cpp")
 
 
 def build_library(verbose: bool = False, extra: list[str] | None = None) -> str:

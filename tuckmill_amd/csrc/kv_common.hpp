@@ -1,0 +1,64 @@
+// What the kernels over the paged key-value cache share (gfx950, wave64): the
+// cache's layout, the visible range of a query and the arguments of the two
+// attention kernels.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <hip/hip_ext.h>
+#include <stdint.h>
+
+#include "q8_common.hpp"
+
+namespace kv {
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// The cache: k [page][kv_head][place][channel], v [page][kv_head][channel][place].
+struct Cache {
+    const void *k, *v;
+    uint32_t pages, page_shift, kv_heads, head_dim;
+    // elements of one page of one head
+    __device__ __forceinline__ size_t head_page() const { return (size_t)head_dim << page_shift; }
+    // first element of a page of a head, in either buffer
+    __device__ __forceinline__ size_t base(uint32_t page, uint32_t head) const {
+        return ((size_t)page * kv_heads + head) * head_page();
+    }
+};
+
+struct AttnArgs {
+    Cache cache;
+    const float *q; // rows from their offset
+    float *out;
+    const uint32_t *table, *lens, *starts; // starts: null, one row per sequence
+    const float *slopes;
+    const uint32_t *first, *prefix;
+    uint32_t tokens, seqs, q_heads, group, table_stride, q_stride, out_stride, window;
+    float scale, softcap;
+};
+
+// Cached tokens of a sequence, cut at what its table can name.
+__device__ __forceinline__ int seq_len(const AttnArgs &a, uint32_t seq) {
+    const uint32_t most = a.table_stride << a.cache.page_shift;
+    const uint32_t len = a.lens[seq];
+    return (int)(len < most ? len : most);
+}
+
+// The positions lo <= j < hi that the query at position p sees.
+__device__ __forceinline__ void visible(const AttnArgs &a, int len, uint32_t seq, uint32_t row, int p,
+                                        int &lo, int &hi) {
+    const uint32_t first = a.first != nullptr ? a.first[row] : 0u;
+    lo = first < (uint32_t)len ? (int)first : len;
+    if (a.window != 0u && p >= 0 && a.window <= (uint32_t)p) {
+        const int from = p - (int)a.window + 1;
+        lo = from > lo ? from : lo;
+    }
+    hi = p + 1;
+    if (a.prefix != nullptr) {
+        const uint32_t prefix = a.prefix[seq];
+        const int both = prefix < (uint32_t)len ? (int)prefix : len;
+        hi = both > hi ? both : hi;
+    }
+    hi = hi < len ? hi : len;
+}
+
+} // namespace kv

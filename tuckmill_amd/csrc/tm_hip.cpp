@@ -24,7 +24,9 @@
 #include <cstdio>
 #include <cstring>
 #include <deque>
+#include <initializer_list>
 #include <mutex>
+#include <new>
 #include <string>
 #include <type_traits>
 #include <unistd.h>
@@ -67,19 +69,30 @@ void alloc_release(Alloc *a) {
 // handle may be freed before end_group and the memory lives on. The references
 // are dropped once the commit (or the recorded step) has taken its own, or when
 // the group is aborted.
-void ops_hold(const Op &op) {
+// Every allocation an operation names, those of its KvParams included.
+template <typename F> void each_alloc(const Op &op, F f) {
     for (int i = 0; i < op.n_alloc; ++i) {
         if (op.a[i] != nullptr) {
-            op.a[i]->refs.fetch_add(1, std::memory_order_relaxed);
+            f(op.a[i]);
+        }
+    }
+    if (op.kv != nullptr) {
+        for (int i = 0; i < op.kv->n_more; ++i) {
+            if (op.kv->more[i] != nullptr) {
+                f(op.kv->more[i]);
+            }
         }
     }
 }
 
+void ops_hold(const Op &op) {
+    each_alloc(op, [](Alloc *a) { a->refs.fetch_add(1, std::memory_order_relaxed); });
+}
+
 void ops_drop(std::vector<Op> &ops) {
     for (const Op &op : ops) {
-        for (int i = 0; i < op.n_alloc; ++i) {
-            alloc_release(op.a[i]);
-        }
+        each_alloc(op, [](Alloc *a) { alloc_release(a); });
+        delete op.kv; // (a recorded operation's own copy)
     }
     ops.clear();
 }
@@ -1241,13 +1254,12 @@ std::vector<Alloc *> allocs_of(tm_hip_ctx *ctx, const std::vector<Op> &ops) {
     const uint64_t keep_epoch = ++ctx->plan_epoch;
     keep.reserve(ops.size() * 3);
     for (const Op &op : ops) {
-        for (int i = 0; i < op.n_alloc; ++i) {
-            Alloc *a = op.a[i];
-            if (a != nullptr && a->keep_epoch != keep_epoch) {
+        each_alloc(op, [&](Alloc *a) {
+            if (a->keep_epoch != keep_epoch) {
                 a->keep_epoch = keep_epoch;
                 keep.push_back(a);
             }
-        }
+        });
     }
     return keep;
 }
@@ -1267,8 +1279,19 @@ int commit_ops(tm_hip_ctx *ctx, const std::vector<Op> &ops, const char *label, c
 int submit(tm_hip_ctx *ctx, Op &op, const char *what, char *err, size_t cap) {
     op.what = what;
     if (ctx->group_active) {
+        if (op.kv != nullptr) { // the caller's parameters end with the call
+            op.kv = new (std::nothrow) KvParams(*op.kv);
+            if (op.kv == nullptr) {
+                return fail(err, cap, TM_HIP_ERR_ALLOC, "%s: recording the operation", what);
+            }
+        }
+        try {
+            ctx->group_ops.push_back(op);
+        } catch (const std::bad_alloc &) {
+            delete op.kv;
+            return fail(err, cap, TM_HIP_ERR_ALLOC, "%s: recording the operation", what);
+        }
         ops_hold(op);
-        ctx->group_ops.push_back(op);
         return TM_HIP_OK;
     }
     char label[kProfileName];
@@ -1631,6 +1654,14 @@ size_t tm_hip_buffer_len(const tm_hip_ctx *ctx, const tm_hip_buffer *buffer) {
     return buffer->len;
 }
 
+void *tm_hip_buffer_contents(const tm_hip_ctx *ctx, const tm_hip_buffer *buffer) {
+    if (ctx == nullptr || buffer == nullptr || buffer->owner != ctx || !buffer->shared ||
+        buffer->alloc->packed) {
+        return nullptr;
+    }
+    return buffer->alloc->ptr;
+}
+
 int tm_hip_buffer_zero(tm_hip_ctx *ctx, tm_hip_buffer *buffer, size_t off, size_t len, char *err,
                        size_t err_cap) {
     if (check_ctx(ctx, err, err_cap, "buffer_zero") != TM_HIP_OK) {
@@ -1984,6 +2015,418 @@ int tm_hip_argmax_f32(tm_hip_ctx *ctx, tm_hip_buffer *x, uint32_t n, tm_hip_buff
     op.extra = n;
     op.y_off = out_index;
     return submit(ctx, op, "argmax_f32", err, err_cap);
+}
+
+// ---- the operators between a step's products --------------------------------
+
+namespace {
+
+int check_operand(tm_hip_ctx *ctx, tm_hip_buffer *b, size_t need, const char *what, const char *role,
+                  char *err, size_t cap) {
+    char name[64];
+    snprintf(name, sizeof name, "%s.%s", what, role);
+    const int rc = check_buffer(ctx, b, need, err, cap, name);
+    if (rc == TM_HIP_OK && b->alloc->packed) {
+        return fail(err, cap, TM_HIP_ERR_UNSUPPORTED, "%s: sealed weight buffer", name);
+    }
+    return rc;
+}
+
+// `rows` rows of `width` f32 from element `off`, `*stride` apart (0: packed, set here).
+int check_rows(tm_hip_ctx *ctx, tm_hip_buffer *b, uint32_t rows, uint32_t width, uint32_t off,
+               uint32_t *stride, const char *what, const char *role, char *err, size_t cap) {
+    if (*stride == 0) {
+        *stride = width;
+    }
+    if (*stride < width) {
+        return fail(err, cap, TM_HIP_ERR_UNSUPPORTED, "%s.%s: rows of %u values %u apart", what, role,
+                    width, *stride);
+    }
+    const size_t need = ((size_t)off + (size_t)(rows - 1u) * *stride + width) * 4u;
+    return check_operand(ctx, b, need, what, role, err, cap);
+}
+
+// Rows of the same buffer that share an element.
+bool rows_overlap(uint32_t rows, uint32_t off_a, uint32_t width_a, uint32_t stride_a, uint32_t off_b,
+                  uint32_t width_b, uint32_t stride_b) {
+    const uint64_t end_a = (uint64_t)off_a + (uint64_t)(rows - 1u) * stride_a + width_a;
+    const uint64_t end_b = (uint64_t)off_b + (uint64_t)(rows - 1u) * stride_b + width_b;
+    if (end_a <= off_b || end_b <= off_a) {
+        return false;
+    }
+    if (stride_a != stride_b) {
+        return true; // interleaved in a way no caller needs
+    }
+    // side by side within one row pitch, like the parts of a fused projection's rows
+    const uint64_t gap = off_b >= off_a ? (uint64_t)(off_b - off_a) % stride_a
+                                        : (stride_a - (uint64_t)(off_a - off_b) % stride_a) % stride_a;
+    return gap < width_a || stride_a - gap < width_b;
+}
+
+// The first of `others` that is `out`'s buffer is a refusal.
+int check_apart(tm_hip_buffer *out, const char *role, std::initializer_list<tm_hip_buffer *> others,
+                const char *what, char *err, size_t cap) {
+    for (tm_hip_buffer *o : others) {
+        if (o != nullptr && o->alloc == out->alloc) {
+            return fail(err, cap, TM_HIP_ERR_UNSUPPORTED,
+                        "%s: the output %s is named as another operand too", what, role);
+        }
+    }
+    return TM_HIP_OK;
+}
+
+int check_cache(tm_hip_ctx *ctx, const tm_hip_kv_cache *c, KvParams *p, const char *what, char *err,
+                size_t cap) {
+    if (c == nullptr) {
+        return fail(err, cap, TM_HIP_ERR_UNSUPPORTED, "%s: null cache", what);
+    }
+    const bool pow2 = c->page_tokens != 0 && (c->page_tokens & (c->page_tokens - 1u)) == 0u;
+    if (c->type_id > 1u || c->pages == 0 || !pow2 || c->page_tokens < 16u || c->page_tokens > 256u ||
+        c->kv_heads == 0 || c->kv_heads > TM_HIP_KV_MAX_HEADS || c->head_dim == 0 ||
+        c->head_dim > 256u || (c->head_dim & 7u) != 0u) {
+        return fail(err, cap, TM_HIP_ERR_UNSUPPORTED,
+                    "%s: cache of type %u (0: F32, 1: F16), %u pages of %u tokens (a power of two, "
+                    "16..256), %u heads (1..%u) of %u channels (a multiple of 8 up to 256)",
+                    what, c->type_id, c->pages, c->page_tokens, c->kv_heads, TM_HIP_KV_MAX_HEADS,
+                    c->head_dim);
+    }
+    // (pages < 2^32, a page at most 2^8 * 2^10 * 2^8 elements: no overflow)
+    const size_t need = (size_t)c->pages * c->page_tokens * c->kv_heads * c->head_dim *
+                        (c->type_id == 1u ? 2u : 4u);
+    int rc;
+    if ((rc = check_operand(ctx, c->k, need, what, "cache.k", err, cap)) != TM_HIP_OK ||
+        (rc = check_operand(ctx, c->v, need, what, "cache.v", err, cap)) != TM_HIP_OK) {
+        return rc;
+    }
+    p->type_id = c->type_id;
+    p->pages = c->pages;
+    p->page_shift = (uint32_t)__builtin_ctz(c->page_tokens);
+    p->kv_heads = c->kv_heads;
+    p->head_dim = c->head_dim;
+    return TM_HIP_OK;
+}
+
+int check_heads(KvParams *p, uint32_t q_heads, const char *what, char *err, size_t cap) {
+    if (q_heads == 0 || q_heads > TM_HIP_KV_MAX_HEADS || q_heads % p->kv_heads != 0) {
+        return fail(err, cap, TM_HIP_ERR_UNSUPPORTED,
+                    "%s: %u query heads (1..%u) over %u key-value heads", what, q_heads,
+                    TM_HIP_KV_MAX_HEADS, p->kv_heads);
+    }
+    p->q_heads = q_heads;
+    return TM_HIP_OK;
+}
+
+void kv_add(KvParams *p, tm_hip_buffer *b) { p->more[p->n_more++] = b != nullptr ? b->alloc : nullptr; }
+
+int submit_kv(tm_hip_ctx *ctx, Op &op, const char *what, char *err, size_t cap) {
+    try {
+        return submit(ctx, op, what, err, cap);
+    } catch (const std::bad_alloc &) {
+        return fail(err, cap, TM_HIP_ERR_ALLOC, "%s: out of host memory", what);
+    }
+}
+
+// Both attention entry points; `starts` is null for one row per sequence.
+int attention(tm_hip_ctx *ctx, const tm_hip_attn *attn, const tm_hip_kv_cache *cache, tm_hip_buffer *q,
+              tm_hip_buffer *table, tm_hip_buffer *lens, tm_hip_buffer *starts, bool ragged,
+              tm_hip_buffer *out, uint32_t tokens, uint32_t seqs, uint32_t q_heads,
+              uint32_t table_stride, uint32_t q_off, uint32_t out_off, uint32_t q_stride,
+              uint32_t out_stride, const char *what, char *err, size_t cap) {
+    if (check_ctx(ctx, err, cap, what) != TM_HIP_OK) {
+        return TM_HIP_ERR_UNSUPPORTED;
+    }
+    KvParams p;
+    int rc = check_cache(ctx, cache, &p, what, err, cap);
+    if (rc == TM_HIP_OK) {
+        rc = check_heads(&p, q_heads, what, err, cap);
+    }
+    if (rc != TM_HIP_OK) {
+        return rc;
+    }
+    if (attn == nullptr || !(attn->scale - attn->scale == 0.0f) ||
+        !(attn->softcap - attn->softcap == 0.0f) || attn->softcap < 0.0f) {
+        return fail(err, cap, TM_HIP_ERR_UNSUPPORTED,
+                    "%s: a finite scale and a finite softcap >= 0 are required", what);
+    }
+    if (seqs == 0 || seqs > TM_HIP_KV_MAX_SEQS || tokens == 0 || tokens > TM_HIP_KV_MAX_TOKENS) {
+        return fail(err, cap, TM_HIP_ERR_UNSUPPORTED, "%s: %u sequences (1..%u), %u rows (1..%u)", what,
+                    seqs, TM_HIP_KV_MAX_SEQS, tokens, TM_HIP_KV_MAX_TOKENS);
+    }
+    if (table_stride == 0 || ((uint64_t)table_stride << p.page_shift) > 0x7fffffffull) {
+        return fail(err, cap, TM_HIP_ERR_UNSUPPORTED,
+                    "%s: a table of %u pages of %u tokens per sequence (1 to 2^31 - 1 positions)", what,
+                    table_stride, 1u << p.page_shift);
+    }
+    const uint32_t width = q_heads * p.head_dim;
+    if ((rc = check_rows(ctx, q, tokens, width, q_off, &q_stride, what, "q", err, cap)) != TM_HIP_OK ||
+        (rc = check_rows(ctx, out, tokens, width, out_off, &out_stride, what, "out", err, cap)) !=
+            TM_HIP_OK ||
+        (rc = check_operand(ctx, table, (size_t)seqs * table_stride * 4u, what, "table", err, cap)) !=
+            TM_HIP_OK ||
+        (rc = check_operand(ctx, lens, (size_t)seqs * 4u, what, "lens", err, cap)) != TM_HIP_OK ||
+        (ragged &&
+         (rc = check_operand(ctx, starts, ((size_t)seqs + 1u) * 4u, what, "starts", err, cap)) !=
+             TM_HIP_OK) ||
+        (attn->slopes != nullptr &&
+         (rc = check_operand(ctx, attn->slopes, (size_t)q_heads * 4u, what, "slopes", err, cap)) !=
+             TM_HIP_OK) ||
+        (attn->first != nullptr &&
+         (rc = check_operand(ctx, attn->first, (size_t)tokens * 4u, what, "first", err, cap)) !=
+             TM_HIP_OK) ||
+        (attn->prefix != nullptr &&
+         (rc = check_operand(ctx, attn->prefix, (size_t)seqs * 4u, what, "prefix", err, cap)) !=
+             TM_HIP_OK) ||
+        (rc = check_apart(out, "out",
+                          {q, cache->k, cache->v, table, lens, starts, attn->slopes, attn->first,
+                           attn->prefix},
+                          what, err, cap)) != TM_HIP_OK) {
+        return rc;
+    }
+    p.tokens = tokens;
+    p.seqs = seqs;
+    p.table_stride = table_stride;
+    p.q_off = q_off;
+    p.out_off = out_off;
+    p.q_stride = q_stride;
+    p.out_stride = out_stride;
+    p.scale = attn->scale;
+    p.softcap = attn->softcap;
+    p.window = attn->window;
+    kv_add(&p, table);
+    kv_add(&p, lens);
+    kv_add(&p, starts);
+    kv_add(&p, attn->slopes);
+    kv_add(&p, attn->first);
+    kv_add(&p, attn->prefix);
+    Op op;
+    op.kind = ragged ? OP_ATTN_PREFILL : OP_ATTN_DECODE;
+    op.a[0] = q->alloc;
+    op.a[1] = cache->k->alloc;
+    op.a[2] = cache->v->alloc;
+    op.a[3] = out->alloc;
+    op.n_alloc = 4;
+    op.writes_mask = 8;
+    op.kv = &p;
+    return submit_kv(ctx, op, what, err, cap);
+}
+
+} // namespace
+
+int tm_hip_rope_store_f32(tm_hip_ctx *ctx, const tm_hip_rope *rope, const tm_hip_kv_cache *cache,
+                          tm_hip_buffer *q, tm_hip_buffer *k, tm_hip_buffer *v,
+                          tm_hip_buffer *q_out, tm_hip_buffer *positions, tm_hip_buffer *slots,
+                          uint32_t tokens, uint32_t q_heads, uint32_t q_off, uint32_t k_off,
+                          uint32_t v_off, uint32_t out_off, uint32_t q_stride, uint32_t k_stride,
+                          uint32_t v_stride, uint32_t out_stride, char *err, size_t err_cap) {
+    static const char what[] = "rope_store";
+    if (check_ctx(ctx, err, err_cap, what) != TM_HIP_OK) {
+        return TM_HIP_ERR_UNSUPPORTED;
+    }
+    KvParams p;
+    int rc = check_cache(ctx, cache, &p, what, err, err_cap);
+    if (rc == TM_HIP_OK) {
+        rc = check_heads(&p, q_heads, what, err, err_cap);
+    }
+    if (rc != TM_HIP_OK) {
+        return rc;
+    }
+    if (tokens == 0 || tokens > TM_HIP_KV_MAX_TOKENS) {
+        return fail(err, err_cap, TM_HIP_ERR_UNSUPPORTED, "%s: %u rows (1..%u)", what, tokens,
+                    TM_HIP_KV_MAX_TOKENS);
+    }
+    uint64_t pairs = 0;
+    if (rope != nullptr && rope->axes >= 1u && rope->axes <= 4u) {
+        for (uint32_t a = 0; a < rope->axes; ++a) {
+            pairs += rope->sections[a];
+        }
+    }
+    if (rope == nullptr || rope->rot_dim == 0 || rope->rot_dim > p.head_dim ||
+        (rope->rot_dim & 1u) != 0u || rope->axes < 1u || rope->axes > 4u ||
+        pairs != rope->rot_dim / 2u) {
+        return fail(err, err_cap, TM_HIP_ERR_UNSUPPORTED,
+                    "%s: an even number of turned channels up to head_dim (%u) and 1 to 4 axes whose "
+                    "sections add up to half of it are required",
+                    what, p.head_dim);
+    }
+    const uint32_t q_width = q_heads * p.head_dim, kv_width = p.kv_heads * p.head_dim;
+    if ((rc = check_rows(ctx, q, tokens, q_width, q_off, &q_stride, what, "q", err, err_cap)) !=
+            TM_HIP_OK ||
+        (rc = check_rows(ctx, k, tokens, kv_width, k_off, &k_stride, what, "k", err, err_cap)) !=
+            TM_HIP_OK ||
+        (rc = check_rows(ctx, v, tokens, kv_width, v_off, &v_stride, what, "v", err, err_cap)) !=
+            TM_HIP_OK ||
+        (rc = check_rows(ctx, q_out, tokens, q_width, out_off, &out_stride, what, "q_out", err,
+                         err_cap)) != TM_HIP_OK ||
+        (rc = check_operand(ctx, positions, (size_t)rope->axes * tokens * 4u, what, "positions", err,
+                            err_cap)) != TM_HIP_OK ||
+        (rc = check_operand(ctx, slots, (size_t)tokens * 4u, what, "slots", err, err_cap)) !=
+            TM_HIP_OK ||
+        (rc = check_operand(ctx, rope->freqs, (size_t)rope->rot_dim / 2u * 4u, what, "freqs", err,
+                            err_cap)) != TM_HIP_OK ||
+        (rc = check_apart(cache->k, "cache.k",
+                          {cache->v, q, k, v, q_out, positions, slots, rope->freqs}, what, err,
+                          err_cap)) != TM_HIP_OK ||
+        (rc = check_apart(cache->v, "cache.v", {q, k, v, q_out, positions, slots, rope->freqs}, what,
+                          err, err_cap)) != TM_HIP_OK ||
+        (rc = check_apart(q_out, "q_out", {positions, slots, rope->freqs}, what, err, err_cap)) !=
+            TM_HIP_OK) {
+        return rc;
+    }
+    const bool in_place = q_out->alloc == q->alloc && out_off == q_off && out_stride == q_stride;
+    if ((q_out->alloc == q->alloc && !in_place &&
+         rows_overlap(tokens, q_off, q_width, q_stride, out_off, q_width, out_stride)) ||
+        (q_out->alloc == k->alloc &&
+         rows_overlap(tokens, k_off, kv_width, k_stride, out_off, q_width, out_stride)) ||
+        (q_out->alloc == v->alloc &&
+         rows_overlap(tokens, v_off, kv_width, v_stride, out_off, q_width, out_stride))) {
+        return fail(err, err_cap, TM_HIP_ERR_UNSUPPORTED,
+                    "%s: rows of q_out overlap rows that the call reads (in place: the offset and "
+                    "stride of q)",
+                    what);
+    }
+    p.tokens = tokens;
+    p.q_off = q_off;
+    p.k_off = k_off;
+    p.v_off = v_off;
+    p.out_off = out_off;
+    p.q_stride = q_stride;
+    p.k_stride = k_stride;
+    p.v_stride = v_stride;
+    p.out_stride = out_stride;
+    p.rot_dim = rope->rot_dim;
+    p.adjacent = rope->adjacent != 0u;
+    uint32_t left[4] = {0, 0, 0, 0};
+    for (uint32_t a = 0; a < rope->axes; ++a) {
+        left[a] = rope->sections[a];
+    }
+    for (uint32_t i = 0, a = 0; i < rope->rot_dim / 2u; ++i) {
+        while (left[a] == 0u) {
+            a = (a + 1u) % rope->axes;
+        }
+        left[a] -= 1u;
+        p.axis[i] = (uint8_t)a;
+        if (rope->interleaved != 0u) {
+            a = (a + 1u) % rope->axes;
+        }
+    }
+    kv_add(&p, cache->k);
+    kv_add(&p, cache->v);
+    kv_add(&p, positions);
+    kv_add(&p, slots);
+    kv_add(&p, rope->freqs);
+    Op op;
+    op.kind = OP_ROPE_STORE;
+    op.a[0] = q->alloc;
+    op.a[1] = k->alloc;
+    op.a[2] = v->alloc;
+    op.a[3] = q_out->alloc;
+    op.n_alloc = 4;
+    op.writes_mask = 8; // (and the cache)
+    op.kv = &p;
+    return submit_kv(ctx, op, what, err, err_cap);
+}
+
+int tm_hip_attn_decode_f32(tm_hip_ctx *ctx, const tm_hip_attn *attn, const tm_hip_kv_cache *cache,
+                           tm_hip_buffer *q, tm_hip_buffer *table, tm_hip_buffer *lens,
+                           tm_hip_buffer *out, uint32_t seqs, uint32_t q_heads,
+                           uint32_t table_stride, uint32_t q_off, uint32_t out_off,
+                           uint32_t q_stride, uint32_t out_stride, char *err, size_t err_cap) {
+    return attention(ctx, attn, cache, q, table, lens, nullptr, false, out, seqs, seqs, q_heads,
+                     table_stride, q_off, out_off, q_stride, out_stride, "attn_decode", err, err_cap);
+}
+
+int tm_hip_attn_prefill_f32(tm_hip_ctx *ctx, const tm_hip_attn *attn, const tm_hip_kv_cache *cache,
+                            tm_hip_buffer *q, tm_hip_buffer *table, tm_hip_buffer *lens,
+                            tm_hip_buffer *starts, tm_hip_buffer *out, uint32_t tokens,
+                            uint32_t seqs, uint32_t q_heads, uint32_t table_stride, uint32_t q_off,
+                            uint32_t out_off, uint32_t q_stride, uint32_t out_stride, char *err,
+                            size_t err_cap) {
+    return attention(ctx, attn, cache, q, table, lens, starts, true, out, tokens, seqs, q_heads,
+                     table_stride, q_off, out_off, q_stride, out_stride, "attn_prefill", err, err_cap);
+}
+
+int tm_hip_logits_adjust_f32(tm_hip_ctx *ctx, const tm_hip_logits_adjust *adjust,
+                             tm_hip_buffer *logits, tm_hip_buffer *out, uint32_t rows,
+                             uint32_t vocab, uint32_t x_off, uint32_t y_off, char *err,
+                             size_t err_cap) {
+    static const char what[] = "logits_adjust";
+    if (check_ctx(ctx, err, err_cap, what) != TM_HIP_OK) {
+        return TM_HIP_ERR_UNSUPPORTED;
+    }
+    if (adjust == nullptr || rows == 0 || rows > TM_HIP_KV_MAX_SEQS || vocab == 0) {
+        return fail(err, err_cap, TM_HIP_ERR_UNSUPPORTED, "%s: %u rows (1..%u) of %u logits", what, rows,
+                    TM_HIP_KV_MAX_SEQS, vocab);
+    }
+    const tm_hip_logits_adjust &a = *adjust;
+    const bool history = a.history != nullptr, biases = a.bias_ids != nullptr;
+    if (history != (a.history_len != nullptr) || history != (a.penalties != nullptr) ||
+        biases != (a.bias_values != nullptr) || biases != (a.bias_len != nullptr)) {
+        return fail(err, err_cap, TM_HIP_ERR_UNSUPPORTED,
+                    "%s: a history comes with its lengths and penalties, biases with their ids, values "
+                    "and lengths",
+                    what);
+    }
+    if ((history && a.history_stride == 0u) || (biases && a.bias_stride == 0u) ||
+        (a.allowed != nullptr && a.allowed_stride < (vocab + 31ull) / 32ull)) {
+        return fail(err, err_cap, TM_HIP_ERR_UNSUPPORTED,
+                    "%s: strides of history %u, biases %u (at least 1) and allowed ids %u words (at "
+                    "least one for 32 of %u)",
+                    what, a.history_stride, a.bias_stride, a.allowed_stride, vocab);
+    }
+    const size_t values = (size_t)rows * vocab;
+    int rc;
+    if ((rc = check_operand(ctx, logits, (x_off + values) * 4u, what, "logits", err, err_cap)) !=
+            TM_HIP_OK ||
+        (rc = check_operand(ctx, out, (y_off + values) * 4u, what, "out", err, err_cap)) != TM_HIP_OK ||
+        (history &&
+         ((rc = check_operand(ctx, a.history, (size_t)rows * a.history_stride * 4u, what, "history", err,
+                              err_cap)) != TM_HIP_OK ||
+          (rc = check_operand(ctx, a.history_len, (size_t)rows * 4u, what, "history_len", err,
+                              err_cap)) != TM_HIP_OK ||
+          (rc = check_operand(ctx, a.penalties, (size_t)rows * 12u, what, "penalties", err, err_cap)) !=
+              TM_HIP_OK)) ||
+        (biases && ((rc = check_operand(ctx, a.bias_ids, (size_t)rows * a.bias_stride * 4u, what,
+                                        "bias_ids", err, err_cap)) != TM_HIP_OK ||
+                    (rc = check_operand(ctx, a.bias_values, (size_t)rows * a.bias_stride * 4u, what,
+                                        "bias_values", err, err_cap)) != TM_HIP_OK ||
+                    (rc = check_operand(ctx, a.bias_len, (size_t)rows * 4u, what, "bias_len", err,
+                                        err_cap)) != TM_HIP_OK)) ||
+        (a.allowed != nullptr &&
+         (rc = check_operand(ctx, a.allowed, (size_t)rows * a.allowed_stride * 4u, what, "allowed", err,
+                             err_cap)) != TM_HIP_OK) ||
+        (rc = check_apart(out, "out",
+                          {a.history, a.history_len, a.penalties, a.bias_ids, a.bias_values, a.bias_len,
+                           a.allowed},
+                          what, err, err_cap)) != TM_HIP_OK) {
+        return rc;
+    }
+    if (out->alloc == logits->alloc && x_off != y_off && x_off < y_off + values && y_off < x_off + values) {
+        return fail(err, err_cap, TM_HIP_ERR_UNSUPPORTED,
+                    "%s: out overlaps the logits (in place: the same offset)", what);
+    }
+    KvParams p;
+    p.q_off = x_off;
+    p.out_off = y_off;
+    p.history_stride = a.history_stride;
+    p.bias_stride = a.bias_stride;
+    p.allowed_stride = a.allowed_stride;
+    kv_add(&p, a.history_len);
+    kv_add(&p, a.penalties);
+    kv_add(&p, a.bias_ids);
+    kv_add(&p, a.bias_values);
+    kv_add(&p, a.bias_len);
+    kv_add(&p, a.allowed);
+    Op op;
+    op.kind = OP_LOGITS;
+    op.a[0] = logits->alloc;
+    op.a[1] = out->alloc;
+    op.a[2] = history ? a.history->alloc : nullptr;
+    op.n_alloc = 3;
+    op.writes_mask = 2;
+    op.rows = rows;
+    op.cols = vocab;
+    op.kv = &p;
+    return submit_kv(ctx, op, what, err, err_cap);
 }
 
 int tm_hip_begin_group(tm_hip_ctx *ctx, char *err, size_t err_cap) {

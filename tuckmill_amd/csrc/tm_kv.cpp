@@ -1,0 +1,121 @@
+// tm_kv.cpp — the operators between a step's products: rotary positions with the
+// store into the paged cache, attention over it, logits. Turns an operation with
+// KvParams (tm_plan.hpp) into kernel arguments, an instantiation and a grid.
+#include "tm_launch.hpp"
+
+#include "kv_attn.hpp"
+#include "kv_logits.hpp"
+#include "kv_rope.hpp"
+
+using namespace tmh;
+
+namespace {
+
+template <typename T> T *ptr_of(const Alloc *a) { return a != nullptr ? (T *)a->ptr : nullptr; }
+
+kv::AttnArgs attn_args(const Op &op) {
+    const KvParams &p = *op.kv;
+    kv::AttnArgs a;
+    a.cache = kv::Cache{op.a[1]->ptr, op.a[2]->ptr, p.pages, p.page_shift, p.kv_heads, p.head_dim};
+    a.q = ptr_of<const float>(op.a[0]) + p.q_off;
+    a.out = ptr_of<float>(op.a[3]) + p.out_off;
+    a.table = ptr_of<const uint32_t>(p.more[0]);
+    a.lens = ptr_of<const uint32_t>(p.more[1]);
+    a.starts = ptr_of<const uint32_t>(p.more[2]);
+    a.slopes = ptr_of<const float>(p.more[3]);
+    a.first = ptr_of<const uint32_t>(p.more[4]);
+    a.prefix = ptr_of<const uint32_t>(p.more[5]);
+    a.tokens = p.tokens;
+    a.seqs = p.seqs;
+    a.q_heads = p.q_heads;
+    a.group = p.q_heads / p.kv_heads;
+    a.table_stride = p.table_stride;
+    a.q_stride = p.q_stride;
+    a.out_stride = p.out_stride;
+    a.window = p.window;
+    a.scale = p.scale;
+    a.softcap = p.softcap;
+    return a;
+}
+
+hipError_t launch_attention(hipStream_t stream, hipEvent_t stop, const Op &op) {
+    const KvParams &p = *op.kv;
+    const kv::AttnArgs args = attn_args(op);
+    const dim3 grid(p.tokens, p.q_heads);
+    if (p.type_id == 1u) {
+        Q8_LAUNCH(kv::attn_rows_kernel<_Float16>, grid, dim3(64), 0, stream, stop, args);
+    } else {
+        Q8_LAUNCH(kv::attn_rows_kernel<float>, grid, dim3(64), 0, stream, stop, args);
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_rope(hipStream_t stream, hipEvent_t stop, const Op &op) {
+    const KvParams &p = *op.kv;
+    kv::RopeArgs a;
+    a.q = ptr_of<const float>(op.a[0]) + p.q_off;
+    a.k = ptr_of<const float>(op.a[1]) + p.k_off;
+    a.v = ptr_of<const float>(op.a[2]) + p.v_off;
+    a.q_out = ptr_of<float>(op.a[3]) + p.out_off;
+    a.k_cache = p.more[0]->ptr;
+    a.v_cache = p.more[1]->ptr;
+    a.positions = ptr_of<const uint32_t>(p.more[2]);
+    a.slots = ptr_of<const uint32_t>(p.more[3]);
+    a.freqs = ptr_of<const float>(p.more[4]);
+    a.tokens = p.tokens;
+    a.q_heads = p.q_heads;
+    a.kv_heads = p.kv_heads;
+    a.head_dim = p.head_dim;
+    a.pages = p.pages;
+    a.page_shift = p.page_shift;
+    a.q_stride = p.q_stride;
+    a.k_stride = p.k_stride;
+    a.v_stride = p.v_stride;
+    a.out_stride = p.out_stride;
+    a.rot_dim = p.rot_dim;
+    a.adjacent = p.adjacent;
+    memcpy(a.axis, p.axis, sizeof a.axis);
+    if (p.type_id == 1u) {
+        Q8_LAUNCH(kv::rope_store_kernel<_Float16>, dim3(p.tokens), dim3(256), 0, stream, stop, a);
+    } else {
+        Q8_LAUNCH(kv::rope_store_kernel<float>, dim3(p.tokens), dim3(256), 0, stream, stop, a);
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_logits(hipStream_t stream, hipEvent_t stop, const Op &op) {
+    const KvParams &p = *op.kv;
+    kv::LogitsArgs a;
+    a.x = ptr_of<const float>(op.a[0]) + p.q_off;
+    a.y = ptr_of<float>(op.a[1]) + p.out_off;
+    a.history = ptr_of<const uint32_t>(op.a[2]);
+    a.history_len = ptr_of<const uint32_t>(p.more[0]);
+    a.penalties = ptr_of<const float>(p.more[1]);
+    a.bias_ids = ptr_of<const uint32_t>(p.more[2]);
+    a.bias_values = ptr_of<const float>(p.more[3]);
+    a.bias_len = ptr_of<const uint32_t>(p.more[4]);
+    a.allowed = ptr_of<const uint32_t>(p.more[5]);
+    a.vocab = op.cols;
+    a.history_stride = p.history_stride;
+    a.bias_stride = p.bias_stride;
+    a.allowed_stride = p.allowed_stride;
+    const uint32_t tiles = (uint32_t)(((uint64_t)op.cols + kv::LOGITS_TILE - 1u) / kv::LOGITS_TILE);
+    Q8_LAUNCH(kv::logits_adjust_kernel, dim3(tiles, op.rows), dim3(256), 0, stream, stop, a);
+    return hipGetLastError();
+}
+
+} // namespace
+
+hipError_t tmdev::launch_kv(hipStream_t stream, hipEvent_t stop, const Op &op) {
+    switch (op.kind) {
+    case OP_ROPE_STORE:
+        return launch_rope(stream, stop, op);
+    case OP_ATTN_DECODE:
+    case OP_ATTN_PREFILL:
+        return launch_attention(stream, stop, op);
+    case OP_LOGITS:
+        return launch_logits(stream, stop, op);
+    default:
+        return hipErrorInvalidValue;
+    }
+}

@@ -760,6 +760,11 @@ hipError_t tmdev::launch_single(hipStream_t stream, hipEvent_t stop, const Op &o
     case OP_QUANT:
         return q8::launch_quantize_act(st, stop, (const float *)op.a[0]->ptr + op.x_off,
                                        (uint8_t *)op.a[1]->ptr, op.cols, op.batch);
+    case OP_ROPE_STORE:
+    case OP_ATTN_DECODE:
+    case OP_ATTN_PREFILL:
+    case OP_LOGITS:
+        return tmdev::launch_kv(st, stop, op);
     default:
         return hipErrorInvalidValue;
     }

@@ -33,6 +33,9 @@ hipError_t launch_list(hipStream_t stream, hipEvent_t stop, const tmh::Launch &l
 hipError_t launch_single(hipStream_t stream, hipEvent_t stop, const tmh::Op &op, uint16_t *split_to,
                          uint32_t split_cols, const tmh::Op *update);
 
+// An operation that carries KvParams (tm_kv.cpp; launch_single's for those kinds).
+hipError_t launch_kv(hipStream_t stream, hipEvent_t stop, const tmh::Op &op);
+
 // dst[0 .. n) = 0 with a fill kernel (not a memset node: the caller may be recording).
 hipError_t zero_words(hipStream_t stream, uint32_t *dst, uint32_t n);
 

@@ -68,7 +68,25 @@ enum OpKind {
     OP_GEMV_LIST, OP_MMA, OP_ROW, OP_ROW_INDIRECT, OP_COPY, OP_PACK, OP_QUANT, OP_I8,
     OP_SCALE, OP_AXPY, OP_SILU_MUL, OP_GELU_MUL, OP_RMSNORM, OP_ARGMAX,
     OP_F16_GEMM, OP_F16_ROW, OP_F16_ROW_INDIRECT, OP_CAST_F16_F32, OP_CAST_F32_F16,
-    OP_CHECKSUM
+    OP_CHECKSUM, OP_ROPE_STORE, OP_ATTN_DECODE, OP_ATTN_PREFILL, OP_LOGITS
+};
+
+// What the operators between a step's products (positions and cache store,
+// attention, logits) carry beyond an Op: more buffers and their numbers. The
+// entry point's own while the call lasts; an operation recorded into a group owns
+// a copy (submit, ops_drop).
+struct KvParams {
+    Alloc *more[6] = {nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
+    int n_more = 0;
+    uint32_t type_id = 0, pages = 0, page_shift = 0, kv_heads = 0, head_dim = 0;
+    uint32_t tokens = 0, seqs = 0, q_heads = 0, table_stride = 0;
+    uint32_t q_off = 0, k_off = 0, v_off = 0, out_off = 0;
+    uint32_t q_stride = 0, k_stride = 0, v_stride = 0, out_stride = 0;
+    float scale = 0.0f, softcap = 0.0f;
+    uint32_t window = 0;
+    uint32_t rot_dim = 0, adjacent = 0;
+    uint8_t axis[128] = {0}; // of every channel pair
+    uint32_t history_stride = 0, bias_stride = 0, allowed_stride = 0;
 };
 
 struct Op {
@@ -81,6 +99,7 @@ struct Op {
     bool packed = false;
     bool shape_label = false;  // profile label carries "<rows>x<cols>"
     const char *what = "";     // static operator name
+    KvParams *kv = nullptr;    // OP_ROPE_STORE, OP_ATTN_*, OP_LOGITS
 };
 
 // Which kernel family and instantiation a recorded product launches with.

@@ -136,6 +136,10 @@ ARGMAX_PARTIAL_BYTES = 512
 CHECKSUM_PARTIAL_BYTES = 8192  # include/tm_hip.h TM_HIP_CHECKSUM_PARTIAL_BYTES
 STAGING_CHUNK_BYTES = 4 << 20  # crates/tuckcore/src/qwen35_gpu.rs:1176
 
+KV_MAX_TOKENS = 1 << 20  # include/tm_hip.h TM_HIP_KV_MAX_TOKENS
+KV_MAX_SEQS = 32768
+KV_MAX_HEADS = 1024
+
 TM_HIP_ERR_NO_DEVICE = -1
 TM_HIP_ERR_SOURCE = -2
 TM_HIP_ERR_ALLOC = -3
@@ -255,6 +259,32 @@ def check_engine_options(kernels: str, profile: str, prefill_batch_given: bool =
                             "--kernels hip for llama-cpu on a GPU")
 
 
+class _KvCacheDesc(ctypes.Structure):  # tm_hip_kv_cache
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("type_id", ctypes.c_uint32),
+                ("pages", ctypes.c_uint32), ("page_tokens", ctypes.c_uint32),
+                ("kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32)]
+
+
+class _RopeDesc(ctypes.Structure):  # tm_hip_rope
+    _fields_ = [("freqs", ctypes.c_void_p), ("rot_dim", ctypes.c_uint32), ("axes", ctypes.c_uint32),
+                ("sections", ctypes.c_uint32 * 4), ("interleaved", ctypes.c_uint32),
+                ("adjacent", ctypes.c_uint32)]
+
+
+class _AttnDesc(ctypes.Structure):  # tm_hip_attn
+    _fields_ = [("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("window", ctypes.c_uint32),
+                ("slopes", ctypes.c_void_p), ("first", ctypes.c_void_p),
+                ("prefix", ctypes.c_void_p)]
+
+
+class _LogitsDesc(ctypes.Structure):  # tm_hip_logits_adjust
+    _fields_ = [("history", ctypes.c_void_p), ("history_len", ctypes.c_void_p),
+                ("penalties", ctypes.c_void_p), ("bias_ids", ctypes.c_void_p),
+                ("bias_values", ctypes.c_void_p), ("bias_len", ctypes.c_void_p),
+                ("allowed", ctypes.c_void_p), ("history_stride", ctypes.c_uint32),
+                ("bias_stride", ctypes.c_uint32), ("allowed_stride", ctypes.c_uint32)]
+
+
 _lib = None
 _lib_lock = threading.Lock()
 
@@ -268,6 +298,7 @@ _SIGS = {
                                             ctypes.c_char_p, ctypes.c_size_t]),
     "tm_hip_buffer_free": (None, [ctypes.c_void_p, ctypes.c_void_p]),
     "tm_hip_buffer_len": (ctypes.c_size_t, [ctypes.c_void_p, ctypes.c_void_p]),
+    "tm_hip_buffer_contents": (ctypes.c_void_p, [ctypes.c_void_p, ctypes.c_void_p]),
     "tm_hip_buffer_zero": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
                                           ctypes.c_size_t, ctypes.c_char_p, ctypes.c_size_t]),
     "tm_hip_upload": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
@@ -307,6 +338,21 @@ _SIGS = {
     "tm_hip_xor_checksum_u32": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32,
                                                ctypes.c_uint32, ctypes.c_void_p, ctypes.c_char_p,
                                                ctypes.c_size_t]),
+    "tm_hip_rope_store_f32": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(_RopeDesc),
+                                             ctypes.POINTER(_KvCacheDesc)] +
+                              [ctypes.c_void_p] * 6 + [ctypes.c_uint32] * 10 +
+                              [ctypes.c_char_p, ctypes.c_size_t]),
+    "tm_hip_attn_decode_f32": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(_AttnDesc),
+                                              ctypes.POINTER(_KvCacheDesc)] +
+                               [ctypes.c_void_p] * 4 + [ctypes.c_uint32] * 7 +
+                               [ctypes.c_char_p, ctypes.c_size_t]),
+    "tm_hip_attn_prefill_f32": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(_AttnDesc),
+                                               ctypes.POINTER(_KvCacheDesc)] +
+                                [ctypes.c_void_p] * 5 + [ctypes.c_uint32] * 8 +
+                                [ctypes.c_char_p, ctypes.c_size_t]),
+    "tm_hip_logits_adjust_f32": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(_LogitsDesc)] +
+                                 [ctypes.c_void_p] * 2 + [ctypes.c_uint32] * 4 +
+                                 [ctypes.c_char_p, ctypes.c_size_t]),
     "tm_hip_begin_group": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t]),
     "tm_hip_end_group": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t]),
     "tm_hip_abort_group": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t]),
@@ -587,6 +633,41 @@ class HipContext:
         words = np.frombuffer(partial.download(0, CHECKSUM_PARTIAL_BYTES), dtype=np.uint32)
         return int(np.bitwise_xor.reduce(words))
 
+    # -- positions, key-value cache, attention, logits ------------------------
+    def rope_store(self, rope: "Rope", cache: "KvCache", q, k, v, q_out, positions, slots,
+                   tokens: int, q_heads: int, q_off=0, k_off=0, v_off=0, out_off=0, q_stride=0,
+                   k_stride=0, v_stride=0, out_stride=0):
+        """q_out = q with rotary positions; k with them and v into the cache at `slots`
+        (0xFFFFFFFF: nowhere). Strides in elements, 0 for packed rows."""
+        self._check_owned(q, k, v, q_out, positions, slots, *rope.buffers, *cache.buffers)
+        self._operate("rope_store", self._lib.tm_hip_rope_store_f32, rope.desc(), cache.desc(),
+                      q.raw, k.raw, v.raw, q_out.raw, positions.raw, slots.raw, tokens, q_heads,
+                      q_off, k_off, v_off, out_off, q_stride, k_stride, v_stride, out_stride)
+
+    def attn_decode(self, attn: "Attention", cache: "KvCache", q, table, lens, out, seqs: int,
+                    q_heads: int, table_stride: int, q_off=0, out_off=0, q_stride=0, out_stride=0):
+        """One query per sequence, at its last cached position."""
+        self._check_owned(q, table, lens, out, *attn.buffers, *cache.buffers)
+        self._operate("attn_decode", self._lib.tm_hip_attn_decode_f32, attn.desc(), cache.desc(),
+                      q.raw, table.raw, lens.raw, out.raw, seqs, q_heads, table_stride, q_off,
+                      out_off, q_stride, out_stride)
+
+    def attn_prefill(self, attn: "Attention", cache: "KvCache", q, table, lens, starts, out,
+                     tokens: int, seqs: int, q_heads: int, table_stride: int, q_off=0, out_off=0,
+                     q_stride=0, out_stride=0):
+        """Rows starts[s]..starts[s+1] of q at the last positions of sequence s."""
+        self._check_owned(q, table, lens, starts, out, *attn.buffers, *cache.buffers)
+        self._operate("attn_prefill", self._lib.tm_hip_attn_prefill_f32, attn.desc(), cache.desc(),
+                      q.raw, table.raw, lens.raw, starts.raw, out.raw, tokens, seqs, q_heads,
+                      table_stride, q_off, out_off, q_stride, out_stride)
+
+    def logits_adjust(self, adjust: "LogitsAdjust", logits, out, rows: int, vocab: int, x_off=0,
+                      y_off=0):
+        """Penalties, biases and the allowed ids of `rows` rows of logits."""
+        self._check_owned(logits, out, *adjust.buffers)
+        self._operate("logits_adjust", self._lib.tm_hip_logits_adjust_f32, adjust.desc(),
+                      logits.raw, out.raw, rows, vocab, x_off, y_off)
+
     # -- additions ---------------------------------------------------------
     def q8_0_pack(self, w, rows: int, cols: int):
         self._check_owned(w)
@@ -702,6 +783,24 @@ class HipBuffer:
         if code != 0:
             raise hip_error(code, err.value.decode(), name)
 
+    def contents(self) -> int:
+        """The device address (tm_hip_buffer_contents): fence before other streams read or
+        fill it, synchronize them before the context uses it again."""
+        address = self._lib.tm_hip_buffer_contents(self._ctx.raw, self.raw) if self.raw else None
+        if not address:
+            raise hip_error(TM_HIP_ERR_UNSUPPORTED, "no device address (freed, private, or sealed "
+                            "weights)", "contents")
+        return int(address)
+
+    @property
+    def __cuda_array_interface__(self) -> dict:
+        """The bytes for array libraries, without a copy: torch.as_tensor(buf, device="cuda")
+        is a uint8 view that lives as long as this handle (and is ordered as `contents` says).
+        torch has to be imported before this module loads the library: both then share the
+        HIP runtime that torch brings along."""
+        return {"shape": (self.len(),), "typestr": "|u1", "data": (self.contents(), False),
+                "version": 2}
+
     def zero(self, offset: int, length: int):
         self._copy("buffer_zero", self._lib.tm_hip_buffer_zero, offset, length)
 
@@ -764,6 +863,89 @@ class HipStep:
             self.free()
         except Exception:
             pass
+
+
+class _Described:
+    """Base of the argument descriptions below: keeps the buffers they name and
+    fills in their handles at each call (a freed one is a null operand there)."""
+
+    def __init__(self, desc, **buffers):
+        self._desc = desc
+        self._named = [(name, b) for name, b in buffers.items() if b is not None]
+        self.buffers = tuple(b for _, b in self._named)
+
+    def desc(self):
+        for name, b in self._named:
+            if b.raw is None:  # (NULL would mean "not given" to the library)
+                raise TuckmillError("InvalidRequest", f"{type(self).__name__}.{name}: the buffer "
+                                    "has been freed", TM_HIP_ERR_UNSUPPORTED)
+            setattr(self._desc, name, b.raw)
+        return ctypes.byref(self._desc)
+
+
+class KvCache(_Described):
+    """A paged key-value cache over two buffers of the caller's (tm_hip_kv_cache):
+    k [page][kv_head][place][channel], v [page][kv_head][channel][place], F16
+    (type_id 1) or F32 (0) elements."""
+
+    def __init__(self, k: HipBuffer, v: HipBuffer, type_id: int, pages: int, page_tokens: int,
+                 kv_heads: int, head_dim: int):
+        super().__init__(_KvCacheDesc(None, None, type_id, pages, page_tokens, kv_heads, head_dim),
+                         k=k, v=v)
+        self.k, self.v = k, v
+        self.type_id, self.pages, self.page_tokens = type_id, pages, page_tokens
+        self.kv_heads, self.head_dim = kv_heads, head_dim
+
+    @staticmethod
+    def plan(type_id: int, pages: int, page_tokens: int, kv_heads: int, head_dim: int) -> int:
+        """Bytes of each of the two buffers."""
+        return pages * page_tokens * kv_heads * head_dim * (2 if type_id == 1 else 4)
+
+    @staticmethod
+    def new(ctx: HipContext, type_id: int, pages: int, page_tokens: int, kv_heads: int,
+            head_dim: int) -> "KvCache":
+        total = KvCache.plan(type_id, pages, page_tokens, kv_heads, head_dim)
+        return KvCache(ctx.buffer(total), ctx.buffer(total), type_id, pages, page_tokens, kv_heads,
+                       head_dim)
+
+
+class Rope(_Described):
+    """Rotary positions (tm_hip_rope): freqs f32 [rot_dim / 2] radians per position,
+    sections[a] channel pairs turned by axis a."""
+
+    def __init__(self, freqs: HipBuffer, rot_dim: int, sections=None, interleaved: bool = False,
+                 adjacent: bool = False):
+        sections = [rot_dim // 2] if sections is None else list(sections)
+        if len(sections) > 4:
+            raise TuckmillError("InvalidRequest", f"{len(sections)} axes: at most 4",
+                                TM_HIP_ERR_UNSUPPORTED)
+        padded = (ctypes.c_uint32 * 4)(*sections)
+        super().__init__(_RopeDesc(None, rot_dim, len(sections), padded, int(interleaved),
+                                   int(adjacent)), freqs=freqs)
+
+
+class Attention(_Described):
+    """What a query sees and how its scores are made (tm_hip_attn): scale, softcap (0:
+    none), window (0: none), slopes f32 [q_heads], first u32 per query row, prefix u32
+    per sequence."""
+
+    def __init__(self, scale: float, softcap: float = 0.0, window: int = 0, slopes=None, first=None,
+                 prefix=None):
+        super().__init__(_AttnDesc(float(scale), float(softcap), window, None, None, None),
+                         slopes=slopes, first=first, prefix=prefix)
+
+
+class LogitsAdjust(_Described):
+    """Penalties for repeated tokens, biases and allowed ids (tm_hip_logits_adjust)."""
+
+    def __init__(self, history=None, history_len=None, penalties=None, bias_ids=None,
+                 bias_values=None, bias_len=None, allowed=None, history_stride: int = 0,
+                 bias_stride: int = 0, allowed_stride: int = 0):
+        super().__init__(_LogitsDesc(None, None, None, None, None, None, None, history_stride,
+                                     bias_stride, allowed_stride),
+                         history=history, history_len=history_len, penalties=penalties,
+                         bias_ids=bias_ids, bias_values=bias_values, bias_len=bias_len,
+                         allowed=allowed)
 
 
 def q8_0_bytes(rows: int, cols: int) -> int:

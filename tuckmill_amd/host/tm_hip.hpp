@@ -225,6 +225,9 @@ class HipBuffer {
     size_t len() const { return raw_ ? tm_hip_buffer_len(ctx_->raw, raw_) : 0; }
     bool is_empty() const { return len() == 0; }
 
+    // Device address (tm_hip_buffer_contents); null for private buffers and sealed weights.
+    void *contents() const { return raw_ ? tm_hip_buffer_contents(ctx_->raw, raw_) : nullptr; }
+
     void zero(size_t offset, size_t length) const {
         call("buffer_zero", [&](char *e) {
             return tm_hip_buffer_zero(ctx_->raw, raw_, offset, length, e, ERR_CAP);
@@ -485,6 +488,50 @@ class HipContext {
                        uint32_t n) const {
         operate("gelu_tanh_mul", [&](char *e) {
             return tm_hip_gelu_tanh_mul_f32(raw(), gate.raw(), up.raw(), out.raw(), n, e, ERR_CAP);
+        });
+    }
+    // -- positions, key-value cache, attention, logits: the C descriptions with raw() handles --
+    void rope_store(const tm_hip_rope &rope, const tm_hip_kv_cache &cache, const HipBuffer &q,
+                    const HipBuffer &k, const HipBuffer &v, const HipBuffer &q_out,
+                    const HipBuffer &positions, const HipBuffer &slots, uint32_t tokens,
+                    uint32_t q_heads, uint32_t q_off = 0, uint32_t k_off = 0, uint32_t v_off = 0,
+                    uint32_t out_off = 0, uint32_t q_stride = 0, uint32_t k_stride = 0,
+                    uint32_t v_stride = 0, uint32_t out_stride = 0) const {
+        operate("rope_store", [&](char *e) {
+            return tm_hip_rope_store_f32(raw(), &rope, &cache, q.raw(), k.raw(), v.raw(), q_out.raw(),
+                                         positions.raw(), slots.raw(), tokens, q_heads, q_off, k_off,
+                                         v_off, out_off, q_stride, k_stride, v_stride, out_stride, e,
+                                         ERR_CAP);
+        });
+    }
+    void attn_decode(const tm_hip_attn &attn, const tm_hip_kv_cache &cache, const HipBuffer &q,
+                     const HipBuffer &table, const HipBuffer &lens, const HipBuffer &out,
+                     uint32_t seqs, uint32_t q_heads, uint32_t table_stride, uint32_t q_off = 0,
+                     uint32_t out_off = 0, uint32_t q_stride = 0, uint32_t out_stride = 0) const {
+        operate("attn_decode", [&](char *e) {
+            return tm_hip_attn_decode_f32(raw(), &attn, &cache, q.raw(), table.raw(), lens.raw(),
+                                          out.raw(), seqs, q_heads, table_stride, q_off, out_off,
+                                          q_stride, out_stride, e, ERR_CAP);
+        });
+    }
+    void attn_prefill(const tm_hip_attn &attn, const tm_hip_kv_cache &cache, const HipBuffer &q,
+                      const HipBuffer &table, const HipBuffer &lens, const HipBuffer &starts,
+                      const HipBuffer &out, uint32_t tokens, uint32_t seqs, uint32_t q_heads,
+                      uint32_t table_stride, uint32_t q_off = 0, uint32_t out_off = 0,
+                      uint32_t q_stride = 0, uint32_t out_stride = 0) const {
+        operate("attn_prefill", [&](char *e) {
+            return tm_hip_attn_prefill_f32(raw(), &attn, &cache, q.raw(), table.raw(), lens.raw(),
+                                           starts.raw(), out.raw(), tokens, seqs, q_heads,
+                                           table_stride, q_off, out_off, q_stride, out_stride, e,
+                                           ERR_CAP);
+        });
+    }
+    void logits_adjust(const tm_hip_logits_adjust &adjust, const HipBuffer &logits,
+                       const HipBuffer &out, uint32_t rows, uint32_t vocab, uint32_t x_off = 0,
+                       uint32_t y_off = 0) const {
+        operate("logits_adjust", [&](char *e) {
+            return tm_hip_logits_adjust_f32(raw(), &adjust, logits.raw(), out.raw(), rows, vocab, x_off,
+                                            y_off, e, ERR_CAP);
         });
     }
     void argmax_f32(const HipBuffer &x, uint32_t n, const HipBuffer &partial, const HipBuffer &out,
