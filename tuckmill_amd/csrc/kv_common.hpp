@@ -7,11 +7,22 @@
 #include <hip/hip_ext.h>
 #include <stdint.h>
 
+#include "kv_plan.hpp"
 #include "q8_common.hpp"
 
 namespace kv {
 
 constexpr float LOG2E = 1.4426950408889634f;
+
+typedef q8::f32x4 f32x4;
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The value of the lane eight columns on, of sixteen.
+__device__ __forceinline__ float ror8(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128, 0xf, 0xf, false));
+}
 
 // The cache: k [page][kv_head][place][channel], v [page][kv_head][channel][place].
 struct Cache {

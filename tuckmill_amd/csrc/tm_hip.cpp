@@ -534,10 +534,10 @@ uint32_t kernel_launches_of(const Launch &l) {
     return (l.bx3_presplit & all) == all ? 1u : 2u; // the split pass, unless nothing is left to it
 }
 
-// Grow the split-float GEMM's workspace to what the largest of the planned
-// launches needs (launches on the context's stream run one after the other and
+// Grow the split-float GEMM's workspace, and the attention's, to what the largest
+// of the planned launches needs (launches on the context's stream run one after the other and
 // share it).
-hipError_t ensure_bx3_workspace(tm_hip_ctx *ctx, const std::vector<Launch> &plan) {
+hipError_t ensure_workspace(tm_hip_ctx *ctx, const std::vector<Launch> &plan) {
     size_t xs = 0, partial = 0;
     for (const Launch &l : plan) {
         if (l.single == nullptr && (l.key.variant == V_BF16X3 || l.key.variant == V_MMA_SPLIT)) {
@@ -565,6 +565,27 @@ hipError_t ensure_bx3_workspace(tm_hip_ctx *ctx, const std::vector<Launch> &plan
     hipError_t e = grow((void **)&ctx->ws.xs, &ctx->ws.xs_bytes, xs);
     if (e == hipSuccess) {
         e = grow((void **)&ctx->ws.partials, &ctx->ws.partial_bytes, partial);
+    }
+    size_t kv_partial = 0, kv_arrival = 0;
+    for (const Launch &l : plan) {
+        if (l.single != nullptr && (l.single->kind == OP_ATTN_DECODE || l.single->kind == OP_ATTN_PREFILL)) {
+            const kv::AttnPlan p = attn_plan_of(*l.single->kv, l.single->kind);
+            kv_partial = p.partial_floats * 4u > kv_partial ? (size_t)(p.partial_floats * 4u) : kv_partial;
+            kv_arrival = p.arrivals * 4u > kv_arrival ? (size_t)(p.arrivals * 4u) : kv_arrival;
+        }
+    }
+    if (e == hipSuccess) {
+        e = grow((void **)&ctx->ws.kv_partials, &ctx->ws.kv_partial_bytes, kv_partial);
+    }
+    if (e == hipSuccess && kv_arrival > ctx->ws.kv_arrival_bytes) {
+        e = grow((void **)&ctx->ws.kv_arrivals, &ctx->ws.kv_arrival_bytes, kv_arrival);
+        if (e == hipSuccess) { // counters start at zero; on the stream, in front of the launch
+            ctx->loose_work = true;
+            e = hipMemsetAsync(ctx->ws.kv_arrivals, 0, ctx->ws.kv_arrival_bytes, ctx->stream);
+            if (e != hipSuccess) {
+                ctx->ws.kv_arrival_bytes = 0; // not usable: allocated again by the next call
+            }
+        }
     }
     return e;
 }
@@ -1153,6 +1174,14 @@ hipError_t issue_launch(tm_hip_ctx *ctx, hipEvent_t stop, const Launch &l) {
     if (l.single == nullptr) {
         return tmdev::launch_list(ctx->stream, stop, l, ctx->ws);
     }
+    if (l.single->kv != nullptr) {
+        KvParams p = *l.single->kv;
+        p.partials = ctx->ws.kv_partials;
+        p.arrivals = ctx->ws.kv_arrivals;
+        Op op = *l.single;
+        op.kv = &p;
+        return tmdev::launch_single(ctx->stream, stop, op, nullptr, 0, nullptr);
+    }
     if (l.split_xs_off >= 0) {
         return tmdev::launch_single(ctx->stream, stop, *l.single,
                                     (uint16_t *)(ctx->ws.xs + l.split_xs_off), l.split_cols, l.update);
@@ -1165,7 +1194,7 @@ hipError_t issue_ops(tm_hip_ctx *ctx, const std::vector<Op> &ops, hipEvent_t sto
                      bool *stop_attached) {
     const std::vector<Launch> plan = plan_launches(ctx, ops);
     *stop_attached = false;
-    hipError_t ws = ensure_bx3_workspace(ctx, plan);
+    hipError_t ws = ensure_workspace(ctx, plan);
     if (ws != hipSuccess) {
         return ws;
     }
@@ -1563,7 +1592,8 @@ void tm_hip_destroy(tm_hip_ctx *ctx) {
         }
     }
     for (void *p : {(void *)ctx->ws.mma_queue, (void *)ctx->ws.mma_partials,
-                    (void *)ctx->ws.arrivals, (void *)ctx->ws.xs, (void *)ctx->ws.partials}) {
+                    (void *)ctx->ws.arrivals, (void *)ctx->ws.xs, (void *)ctx->ws.partials,
+                    (void *)ctx->ws.kv_partials, (void *)ctx->ws.kv_arrivals}) {
         if (p != nullptr) {
             (void)hipFree(p);
         }
@@ -2489,7 +2519,7 @@ int tm_hip_end_group_recorded(tm_hip_ctx *ctx, tm_hip_step **out, char *err, siz
     step->owner = ctx;
     step->operators = (uint32_t)ops.size();
     const std::vector<Launch> plan = plan_launches(ctx, ops);
-    hipError_t e = ensure_bx3_workspace(ctx, plan); // allocates: before the stream records
+    hipError_t e = ensure_workspace(ctx, plan); // allocates: before the stream records
     if (e != hipSuccess) {
         delete step;
         return hip_fail(err, err_cap, "end_group_recorded: workspace", e);

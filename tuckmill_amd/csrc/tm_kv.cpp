@@ -4,6 +4,7 @@
 #include "tm_launch.hpp"
 
 #include "kv_attn.hpp"
+#include "kv_attn_decode.hpp"
 #include "kv_logits.hpp"
 #include "kv_rope.hpp"
 
@@ -48,6 +49,35 @@ hipError_t launch_attention(hipStream_t stream, hipEvent_t stop, const Op &op) {
         Q8_LAUNCH(kv::attn_rows_kernel<float>, grid, dim3(64), 0, stream, stop, args);
     }
     return hipGetLastError();
+}
+
+template <typename T, int D, int W>
+hipError_t launch_decode_as(hipStream_t stream, hipEvent_t stop, const kv::DecodeArgs &args) {
+    const dim3 grid(args.a.cache.kv_heads * args.head_tiles * args.splits, args.a.seqs);
+    if (args.a.cache.head_dim == (uint32_t)D) {
+        Q8_LAUNCH((kv::attn_decode_kernel<T, D, true, W>), grid, dim3(256), 0, stream, stop, args);
+    } else {
+        Q8_LAUNCH((kv::attn_decode_kernel<T, D, false, W>), grid, dim3(256), 0, stream, stop, args);
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_decode(hipStream_t stream, hipEvent_t stop, const Op &op) {
+    const KvParams &p = *op.kv;
+    const kv::AttnPlan plan = attn_plan_of(p, op.kind);
+    if (plan.splits > 1u && (p.partials == nullptr || p.arrivals == nullptr)) {
+        return hipErrorInvalidValue;
+    }
+    const kv::DecodeArgs args{attn_args(op), p.partials, p.arrivals, plan.splits, plan.head_tiles};
+    const uint32_t d = p.head_dim;
+    if (p.type_id == 1u) {
+        return d <= 64u    ? launch_decode_as<_Float16, 64, 4>(stream, stop, args)
+               : d <= 128u ? launch_decode_as<_Float16, 128, 3>(stream, stop, args)
+                           : launch_decode_as<_Float16, 256, 2>(stream, stop, args);
+    }
+    return d <= 64u    ? launch_decode_as<float, 64, 3>(stream, stop, args)
+           : d <= 128u ? launch_decode_as<float, 128, 2>(stream, stop, args)
+                       : launch_decode_as<float, 256, 1>(stream, stop, args);
 }
 
 hipError_t launch_rope(hipStream_t stream, hipEvent_t stop, const Op &op) {
@@ -111,6 +141,7 @@ hipError_t tmdev::launch_kv(hipStream_t stream, hipEvent_t stop, const Op &op) {
     case OP_ROPE_STORE:
         return launch_rope(stream, stop, op);
     case OP_ATTN_DECODE:
+        return launch_decode(stream, stop, op);
     case OP_ATTN_PREFILL:
         return launch_attention(stream, stop, op);
     case OP_LOGITS:

@@ -12,6 +12,7 @@
 #include <cstring>
 #include <type_traits>
 
+#include "kv_plan.hpp"
 #include "q8_plan.hpp"
 #include "tm_hip.h"
 
@@ -51,6 +52,12 @@ struct Workspace {
     float *partials = nullptr;
     size_t partial_bytes = 0;
     uint32_t *arrivals = nullptr;
+    // Attention whose positions are shared between workgroups: partial results and
+    // arrival counters (zero between launches).
+    float *kv_partials = nullptr;
+    size_t kv_partial_bytes = 0;
+    uint32_t *kv_arrivals = nullptr;
+    size_t kv_arrival_bytes = 0;
 };
 
 struct Alloc {
@@ -87,7 +94,17 @@ struct KvParams {
     uint32_t rot_dim = 0, adjacent = 0;
     uint8_t axis[128] = {0}; // of every channel pair
     uint32_t history_stride = 0, bias_stride = 0, allowed_stride = 0;
+    float *partials = nullptr; // of the context's workspace, filled in when the launch is issued
+    uint32_t *arrivals = nullptr;
 };
+
+inline kv::AttnPlan attn_plan_of(const KvParams &p, OpKind kind) {
+    if (kind == OP_ATTN_DECODE) {
+        return kv::decode_plan(p.type_id, p.seqs, p.q_heads, p.kv_heads, p.head_dim,
+                               (uint64_t)p.table_stride << p.page_shift);
+    }
+    return kv::AttnPlan{};
+}
 
 struct Op {
     OpKind kind;
