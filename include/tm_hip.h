@@ -367,7 +367,8 @@ int tm_hip_rope_store_f32(tm_hip_ctx *ctx, const tm_hip_rope *rope, const tm_hip
  *     slopes: x -= slopes[h] * |p - j|
  * out = sum_j softmax(x)_j * v_j. Where nothing is visible, or every visible
  * score is -infinity, out is zero. What is cached at positions a query does not
- * see has no influence on it, infinities and NaN included. Scores, softmax
+ * see has no influence on it, infinities and NaN included (an infinite key or value
+ * that it does see may make its result NaN). Scores, softmax
  * statistics and sums are f32; over F16 pages q and the softmax weights enter the
  * matrix products as the sum of two f16 numbers (22 bits), not rounded to one.
  * slopes (f32 [q_heads]), first (u32, one per query row: where its document
@@ -384,7 +385,7 @@ typedef struct tm_hip_attn {
  * Position j lies in page table[s * table_stride + j / page_tokens] at place
  * j % page_tokens; positions in pages that are not in the cache are not
  * visible, and lens is cut at table_stride * page_tokens (which is at most
- * 2^31 - 1). Rows of q and out are q_heads * head_dim values from q_off, out_off,
+ * 2^30). Rows of q and out are q_heads * head_dim values from q_off, out_off,
  * strides of 0 mean packed. q_heads is a multiple of kv_heads. A long sequence is
  * split over workgroups and joined in the same launch, in the order of
  * positions: the same call gives the same bits. */
@@ -397,9 +398,10 @@ int tm_hip_attn_decode_f32(tm_hip_ctx *ctx, const tm_hip_attn *attn, const tm_hi
 /* A ragged batch of query rows: rows starts[s] .. starts[s + 1] (of `tokens`;
  * starts has seqs + 1 entries and ascends) are the last positions of sequence s,
  * whose lens[s] cached tokens include them (tm_hip_rope_store_f32 has stored
- * them). Rows in no sequence (behind starts[seqs], or of a sequence whose
- * bounds do not ascend within `tokens`) keep what out held. Otherwise as
- * tm_hip_attn_decode_f32; attn->first has an entry per row. */
+ * them). Rows in no sequence keep what out held: those behind starts[seqs], and
+ * those of a sequence whose two bounds do not ascend within `tokens`, or whose
+ * first is below an earlier entry. Otherwise as tm_hip_attn_decode_f32;
+ * attn->first has an entry per row. */
 int tm_hip_attn_prefill_f32(tm_hip_ctx *ctx, const tm_hip_attn *attn, const tm_hip_kv_cache *cache,
                             tm_hip_buffer *q, tm_hip_buffer *table, tm_hip_buffer *lens,
                             tm_hip_buffer *starts, tm_hip_buffer *out, uint32_t tokens,

@@ -46,8 +46,7 @@ template <int D, bool FULL> struct Tile<_Float16, D, FULL> {
         }
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        const int e = top < INFINITY ? 13 - (int)((__float_as_uint(top) >> 23) & 0xffu) + 127 : 0;
-        const int by = e < 100 ? e : 100;
+        const int by = scale_bits(top);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
 #pragma unroll
@@ -286,7 +285,7 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_decode_kernel(Decode
         if (a.softcap > 0.0f) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                x[j] = cap_log2 * tanhf(x[j] * to_log2);
+                x[j] = cap_log2 * tanh_of(x[j] * to_log2);
             }
         } else {
 #pragma unroll

@@ -1,0 +1,640 @@
+// Attention of ragged batches of query rows over the paged cache.
+#pragma once
+
+#include "kv_attn_decode.hpp"
+
+namespace kv {
+
+struct PrefillArgs {
+    AttnArgs a;
+    float *partials;
+    uint32_t *arrivals;
+    uint32_t splits, tile_bound;
+};
+
+// Sizes of the kernel for pages of T and heads of up to D channels. A row is a query
+// and a head; heads of one key-value head that belong to the same query are
+// neighbours, so a tile of rows reads its keys and values once for all of them.
+template <typename T, int D> struct PrefillShape {
+    static constexpr int E = 16 / (int)sizeof(T);   // elements of a 16-byte unit
+    static constexpr int N = 128 / (int)sizeof(T);  // positions of a step: 64 or 32
+    static constexpr int SUB = N / 32;              // tiles of scores
+    static constexpr int UK = D / E;                // units of a key
+    static constexpr int KS = UK / 2;               // operand pieces of a key
+    static constexpr int DT = D / 32;               // channel tiles
+    static constexpr int BYTES = N * D * (int)sizeof(T); // of a step's keys, and of its values
+    static constexpr int FETCHES = BYTES / 1024 / 4;     // a wave's, of either
+    static constexpr int SWIZZLE = UK < 16 ? UK - 1 : 15;
+};
+
+// 64 x 16 bytes from the lanes' addresses into 1 KiB of LDS. From inline assembly, and
+// waited for by hand: the compiler's own bookkeeping would order every LDS read
+// behind all such loads in flight.
+__device__ __forceinline__ void fetch16(const void *from, const uint8_t *lds) {
+    const uint32_t m = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m), "v"(from) : "memory", "m0");
+}
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// What differs between the two types of page: how a row's q is held, the products
+// and how weights enter the second one.
+template <typename T, int D> struct Rows;
+
+template <int D> struct Rows<_Float16, D> {
+    typedef PrefillShape<_Float16, D> S;
+    typedef f16x8 Unit;
+    Unit hi[S::KS], lo[S::KS]; // q in two parts (22 bits of the row's largest magnitude)
+
+    __device__ __forceinline__ float load_q(const float *row, uint32_t h, uint32_t hd, bool live) {
+        float top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < S::KS; ++s) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t d = 8u * (2u * s + h) + j;
+                top = fmaxf(top, live && d < hd ? fabsf(row[d]) : 0.0f);
+            }
+        }
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const int by = scale_bits(top);
+#pragma unroll
+        for (int s = 0; s < S::KS; ++s) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t d = 8u * (2u * s + h) + j;
+                const float y = live && d < hd ? ldexpf(row[d], by) : 0.0f;
+                hi[s][j] = (_Float16)y;
+                const float whole = (float)hi[s][j];
+                lo[s][j] = (_Float16)(fabsf(whole) < INFINITY ? y - whole : 0.0f);
+            }
+        }
+        return ldexpf(1.0f, -by);
+    }
+    __device__ __forceinline__ f32x16 score(f32x16 acc, const Unit &k, int s) const {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, hi[s], acc, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(k, lo[s], acc, 0, 0, 0);
+    }
+    static constexpr int PIECES = S::N / 16; // of the weights: 16 positions each
+    struct Weights {
+        Unit hi[PIECES], lo[PIECES];
+    };
+    static __device__ __forceinline__ void pack(Weights &w, const float (&x)[S::SUB][16]) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float y = x[i / 2][(i % 2) * 8 + j];
+                w.hi[i][j] = (_Float16)y;
+                w.lo[i][j] = (_Float16)(y - (float)w.hi[i][j]);
+            }
+        }
+    }
+    static __device__ __forceinline__ f32x16 weigh(f32x16 acc, const Unit &v, const Weights &w, int i) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w.hi[i], acc, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w.lo[i], acc, 0, 0, 0);
+    }
+    // unit of a channel's positions that piece i takes for lane half h
+    static __device__ __forceinline__ uint32_t v_unit(int i, uint32_t h) { return 2u * i + h; }
+};
+
+template <int D> struct Rows<float, D> {
+    typedef PrefillShape<float, D> S;
+    typedef f32x4 Unit;
+    Unit q[S::KS];
+
+    __device__ __forceinline__ float load_q(const float *row, uint32_t h, uint32_t hd, bool live) {
+#pragma unroll
+        for (int s = 0; s < S::KS; ++s) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t d = 4u * (2u * s + h) + j;
+                q[s][j] = live && d < hd ? row[d] : 0.0f;
+            }
+        }
+        return 1.0f;
+    }
+    __device__ __forceinline__ f32x16 score(f32x16 acc, const Unit &k, int s) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(k[j], q[s][j], acc, 0, 0, 0);
+        }
+        return acc;
+    }
+    static constexpr int PIECES = 4; // of the weights: 4 positions for each half
+    struct Weights {
+        float x[16];
+    };
+    static __device__ __forceinline__ void pack(Weights &w, const float (&x)[S::SUB][16]) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+            w.x[v] = x[0][v];
+        }
+    }
+    static __device__ __forceinline__ f32x16 weigh(f32x16 acc, const Unit &v, const Weights &w, int i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(v[j], w.x[4 * i + j], acc, 0, 0, 0);
+        }
+        return acc;
+    }
+    static __device__ __forceinline__ uint32_t v_unit(int i, uint32_t h) { return (i / 2) * 4u + 2u * h + (i % 2); }
+};
+
+// A workgroup of four waves per key-value head, tile of 128 rows and share of the
+// positions; each wave has 32 rows and reads the step's keys and values from LDS,
+// where the four fetch them straight from the pages, a step ahead. The products run
+// transposed like the decode kernel's, S^T = K q^T in 32 x 32 tiles whose rows the
+// positions are dealt to (row 8 a + 4 h + b of a tile is position
+// 16 (a / 2) + 8 h + 4 (a % 2) + b) such that a lane holds of S^T what it hands to O^T = V^T P.
+// In LDS the 16-byte units of a row are swapped by exclusive or with the row's number,
+// which spreads a column of units over the banks.
+template <typename T, int D, bool FULL, int WAVES_PER_SIMD>
+__global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(PrefillArgs args) {
+    typedef PrefillShape<T, D> S;
+    typedef Rows<T, D> R;
+    typedef typename R::Unit Unit;
+    extern __shared__ __align__(16) uint8_t lds[]; // two stages of keys and values
+    __shared__ int range[4][2];
+    __shared__ uint32_t arrived;
+    const AttnArgs &a = args.a;
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t c = lane & 31u, h = lane >> 5;
+    const uint32_t kvh = blockIdx.x % a.cache.kv_heads, rest = blockIdx.x / a.cache.kv_heads;
+    const uint32_t split = rest % args.splits, index = rest / args.splits;
+    const uint32_t hd = FULL ? (uint32_t)D : a.cache.head_dim, shift = a.cache.page_shift;
+
+    // The tile this workgroup has: the sequences' tiles one after the other, the last
+    // (with the most positions to see) first.
+    // (A sequence has rows where its bounds ascend within the batch and no earlier
+    // bound is above its first, so that no two sequences share one.)
+    uint32_t seq = 0, tile = 0, row0 = 0, rows = 0, want = 0xffffffffu;
+    for (int pass = 0; pass < 2; ++pass) {
+        uint32_t before = 0, highest = 0;
+        bool here = false;
+        for (uint32_t s0 = 0; s0 < a.seqs && !here; s0 += 64u) {
+            const uint32_t s = min(s0 + lane, a.seqs - 1u);
+            const uint32_t r0 = a.starts[s], r1 = a.starts[s + 1u];
+            uint32_t above = r0;
+            for (uint32_t x = 1; x < 64u; x <<= 1) {
+                const uint32_t y = __shfl_up(above, x);
+                above = lane >= x ? max(above, y) : above;
+            }
+            above = max(above, highest);
+            highest = __shfl(above, 63);
+            const bool there = s0 + lane < a.seqs && r0 == above && r0 <= r1 && r1 <= a.tokens;
+            const uint32_t n = there ? (r1 - r0) * a.group : 0u, mine = (n + 127u) >> 7;
+            uint32_t upto = mine;
+            for (uint32_t x = 1; x < 64u; x <<= 1) {
+                const uint32_t y = __shfl_up(upto, x);
+                upto += lane >= x ? y : 0u;
+            }
+            if (pass == 1) {
+                const uint64_t found = __ballot(want < before + upto);
+                if (found != 0ull) {
+                    const int at = __builtin_ctzll(found);
+                    seq = s0 + (uint32_t)at;
+                    tile = want - before - (__shfl(upto, at) - __shfl(mine, at));
+                    row0 = __shfl(r0, at);
+                    rows = __shfl(n, at);
+                    here = true;
+                }
+            }
+            before += __shfl(upto, 63);
+        }
+        if (pass == 0) {
+            if (index >= before) {
+                return;
+            }
+            want = before - 1u - index;
+        }
+    }
+    seq = __builtin_amdgcn_readfirstlane(seq);
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    row0 = __builtin_amdgcn_readfirstlane(row0);
+    rows = __builtin_amdgcn_readfirstlane(rows);
+
+    // this lane's row
+    const int len = seq_len(a, seq), n = (int)(rows / a.group);
+    const uint32_t r = tile * 128u + wave * 32u + c;
+    const bool live = r < rows;
+    const uint32_t query = live ? r / a.group : 0u, head = kvh * a.group + (live ? r % a.group : 0u);
+    const uint32_t row = row0 + query;
+    const int p = len - n + (int)query;
+    int lo = 0, hi = 0;
+    if (live) {
+        visible(a, len, seq, row, p, lo, hi);
+    }
+    // What any row of the wave sees, and what all of them see. (Rows that are not
+    // there may be given anything.)
+    const bool sees = live && lo < hi;
+    int any_lo = sees ? lo : 0x7fffffff, any_hi = sees ? hi : 0, all_lo = live ? lo : 0, all_hi = live ? hi : 0x7fffffff;
+    for (int x = 32; x > 0; x >>= 1) {
+        any_lo = min(any_lo, __shfl_xor(any_lo, x));
+        any_hi = max(any_hi, __shfl_xor(any_hi, x));
+        all_lo = max(all_lo, __shfl_xor(all_lo, x));
+        all_hi = min(all_hi, __shfl_xor(all_hi, x));
+    }
+    any_lo = __builtin_amdgcn_readfirstlane(any_lo);
+    any_hi = __builtin_amdgcn_readfirstlane(any_hi);
+    all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+    all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+    if (lane == 0u) {
+        range[wave][0] = any_lo;
+        range[wave][1] = any_hi;
+    }
+    __syncthreads();
+    const int from = min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0]));
+    const int upto = max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1]));
+    const uint32_t start = __builtin_amdgcn_readfirstlane(from < upto ? (uint32_t)from & ~(uint32_t)(S::N - 1) : 0u);
+    const uint32_t steps = __builtin_amdgcn_readfirstlane(from < upto ? ((uint32_t)upto - start + S::N - 1u) / S::N : 0u);
+    const uint32_t per = (steps + args.splits - 1u) / args.splits;
+    const uint32_t parts = per != 0u ? (steps + per - 1u) / per : 1u;
+    if (split >= parts) {
+        return;
+    }
+    const uint32_t s_begin = split * per, s_end = min(steps, s_begin + per);
+
+    R q;
+    const float unscale = q.load_q(a.q + (size_t)row * a.q_stride + (size_t)head * hd, h, hd, live);
+    const float slope = a.slopes != nullptr ? a.slopes[head] * LOG2E : 0.0f;
+    const float to_log2 = a.softcap > 0.0f ? a.scale * unscale / a.softcap : a.scale * unscale * LOG2E;
+    const float cap_log2 = a.softcap * LOG2E;
+
+    // Pages of a step: one for every 16 positions.
+    constexpr int PAGES = S::N / 16;
+    const __attribute__((address_space(4))) uint32_t *table =
+        (const __attribute__((address_space(4))) uint32_t *)(a.table + (size_t)seq * a.table_stride);
+    const uint32_t last_entry = a.table_stride - 1u, in_page = (1u << shift) - 1u;
+    const uint32_t page_elements = hd << shift;
+    uint32_t pages[PAGES], next_pages[PAGES];
+    auto look_up = [&](uint32_t step) {
+        const uint32_t base = start + step * S::N;
+#pragma unroll
+        for (int i = 0; i < PAGES; ++i) {
+            next_pages[i] = table[min((base + 16u * i) >> shift, last_entry)];
+        }
+    };
+    // Fetch a step: a wave's keys lie within 16 positions, a lane's values within one unit.
+    const uint32_t v_at = ((lane & 7u) ^ (lane >> 3)) * S::E;
+    auto fetch = [&](uint32_t step, uint32_t stage) {
+        const uint32_t base = start + step * S::N;
+        uint8_t *k_lds = lds + stage * (2u * S::BYTES) + wave * (S::FETCHES * 1024u);
+        uint8_t *v_lds = k_lds + S::BYTES;
+        uint32_t k_page = next_pages[0], v_page = next_pages[0];
+#pragma unroll
+        for (int i = 1; i < PAGES; ++i) {
+            k_page = (wave * (S::N / 4u)) >> 4 == (uint32_t)i ? next_pages[i] : k_page;
+            v_page = v_at >> 4 == (uint32_t)i ? next_pages[i] : v_page;
+        }
+        k_page = k_page < a.cache.pages ? k_page : 0u; // (not seen by any row; somewhere to read from)
+        v_page = v_page < a.cache.pages ? v_page : 0u;
+        const T *k = (const T *)a.cache.k + ((size_t)k_page * a.cache.kv_heads + kvh) * page_elements;
+        const T *v = (const T *)a.cache.v + ((size_t)v_page * a.cache.kv_heads + kvh) * page_elements +
+                     ((base + v_at) & in_page);
+#pragma unroll
+        for (int f = 0; f < S::FETCHES; ++f) {
+            const uint32_t i = wave * S::FETCHES + f;
+            const uint32_t at = i * (64u / S::UK) + lane / S::UK; // row of the stage
+            const uint32_t unit = (lane % S::UK) ^ (at & S::SWIZZLE);
+            const uint32_t position = (at & ~12u) | (at & 4u) << 1 | (at & 8u) >> 1;
+            const uint32_t d = unit * S::E;
+            fetch16(k + ((base + position) & in_page) * hd + (FULL || d < hd ? d : 0u), k_lds + f * 1024);
+        }
+#pragma unroll
+        for (int f = 0; f < S::FETCHES; ++f) {
+            const uint32_t d = (wave * S::FETCHES + f) * 8u + (lane >> 3);
+            fetch16(v + ((FULL ? d : min(d, hd - 1u)) << shift), v_lds + f * 1024);
+        }
+    };
+
+    f32x16 o[S::DT];
+#pragma unroll
+    for (int t = 0; t < S::DT; ++t) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+            o[t][v] = 0.0f;
+        }
+    }
+    float top = -3.402823466e38f, l = 0.0f;
+    bool left_out = false;
+    if (s_begin < s_end) {
+        look_up(s_begin);
+        fetch(s_begin, 0u);
+    }
+    for (uint32_t step = s_begin; step < s_end; ++step) {
+#pragma unroll
+        for (int i = 0; i < PAGES; ++i) {
+            pages[i] = next_pages[i];
+        }
+        if (step + 1u < s_end) {
+            look_up(step + 1u);
+        }
+        // This wave's fetches have landed and its reads of the other stage are done;
+        // behind the barrier everybody's.
+        __builtin_amdgcn_s_waitcnt(7 << 4); // vmcnt(0) lgkmcnt(0)
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const uint32_t stage = (step - s_begin) & 1u;
+        if (step + 1u < s_end) {
+            fetch(step + 1u, stage ^ 1u);
+        }
+        const int base = (int)(start + step * S::N);
+        if (base >= any_hi || base + S::N <= any_lo) {
+            continue; // nothing for this wave's rows
+        }
+        const uint8_t *k_lds = lds + stage * (2u * S::BYTES), *v_lds = k_lds + S::BYTES;
+        f32x16 acc[S::SUB];
+#pragma unroll
+        for (int b = 0; b < S::SUB; ++b) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                acc[b][v] = 0.0f;
+            }
+        }
+        // (each piece's reads stand before the products of the one in front of it and no
+        // earlier: left alone, the compiler reads everything first and spills)
+        Unit k_next[S::SUB];
+        auto read_k = [&](int s) {
+#pragma unroll
+            for (int b = 0; b < S::SUB; ++b) {
+                const uint32_t at = 32u * b + c, unit = 2u * s + h;
+                const Unit k = *(const Unit *)(k_lds + (at * S::UK + (unit ^ (at & S::SWIZZLE))) * 16u);
+                k_next[b] = !FULL && unit * S::E >= hd ? Unit{} : k;
+            }
+        };
+        read_k(0);
+#pragma unroll
+        for (int s = 0; s < S::KS; ++s) {
+            Unit k[S::SUB];
+#pragma unroll
+            for (int b = 0; b < S::SUB; ++b) {
+                k[b] = k_next[b];
+            }
+            asm volatile("" ::: "memory");
+            if (s + 1 < S::KS) {
+                read_k(s + 1);
+            }
+#pragma unroll
+            for (int b = 0; b < S::SUB; ++b) {
+                acc[b] = q.score(acc[b], k[b], s);
+            }
+        }
+        float x[S::SUB][16];
+        const int mine = base + 8 * (int)h; // position of value v of tile b: mine + 32 b + 16 (v / 8) + v % 8
+        if (a.softcap > 0.0f) {
+#pragma unroll
+            for (int b = 0; b < S::SUB; ++b) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    x[b][v] = cap_log2 * tanh_of(acc[b][v] * to_log2);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int b = 0; b < S::SUB; ++b) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    x[b][v] = acc[b][v] * to_log2;
+                }
+            }
+        }
+        if (a.slopes != nullptr) {
+#pragma unroll
+            for (int b = 0; b < S::SUB; ++b) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    x[b][v] -= slope * fabsf((float)(p - mine - (32 * b + 16 * (v / 8) + v % 8)));
+                }
+            }
+        }
+        bool known = true;
+#pragma unroll
+        for (int i = 0; i < PAGES; ++i) {
+            known = known && pages[i] < a.cache.pages;
+        }
+        const bool whole = known && base >= all_lo && base + S::N <= all_hi;
+        if (!whole) {
+#pragma unroll
+            for (int b = 0; b < S::SUB; ++b) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const int at = mine + 32 * b + 16 * (v / 8) + v % 8;
+                    const bool seen = at >= lo && at < hi && pages[2 * b + v / 8] < a.cache.pages;
+                    x[b][v] = seen ? x[b][v] : -INFINITY;
+                }
+            }
+        }
+        float most = x[0][0];
+#pragma unroll
+        for (int b = 0; b < S::SUB; ++b) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                most = fmaxf(most, x[b][v]);
+            }
+        }
+        if (__any(most > top + 8.0f)) {
+            most = fmaxf(most, __shfl_xor(most, 32));
+            most = fmaxf(most, top);
+            const float keep = exp2_of(top - most);
+            top = most;
+            l *= keep;
+#pragma unroll
+            for (int t = 0; t < S::DT; ++t) {
+                o[t] *= keep;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < S::SUB; ++b) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                x[b][v] = exp2_of(x[b][v] - top + 6.0f);
+                l += x[b][v];
+            }
+        }
+        typename R::Weights w;
+        R::pack(w, x);
+        auto v_of = [&](int t, int i) {
+            const uint32_t d = 32u * t + c, unit = R::v_unit(i, h);
+            return *(const Unit *)(v_lds + (d * 8u + (unit ^ (d & 7u))) * 16u);
+        };
+        if (!whole) {
+            // A value that is not finite must not reach a row that does not see it through
+            // a weight of zero: such a step's values are added after the loop.
+            float bad = 0.0f;
+#pragma unroll
+            for (int t = 0; t < S::DT; ++t) {
+#pragma unroll
+                for (int i = 0; i < R::PIECES; ++i) {
+                    asm volatile("" ::: "memory");
+                    const Unit v = v_of(t, i);
+#pragma unroll
+                    for (int j = 0; j < S::E; ++j) {
+                        bad += 0.0f * (float)v[j];
+                    }
+                }
+            }
+            if (__any(bad != 0.0f)) {
+                left_out = true;
+                continue;
+            }
+        }
+        Unit v_next = v_of(0, 0);
+#pragma unroll
+        for (int i = 0; i < R::PIECES * S::DT; ++i) {
+            const Unit v = v_next;
+            asm volatile("" ::: "memory");
+            if (i + 1 < R::PIECES * S::DT) {
+                v_next = v_of((i + 1) % S::DT, (i + 1) / S::DT);
+            }
+            o[i % S::DT] = R::weigh(o[i % S::DT], v, w, i / S::DT);
+        }
+    }
+    if (left_out) {
+        // The steps in which the wave met a value that is not finite, found again the way the
+        // loop found them, position by position: rare, and as slow as it looks.
+        const float *q_row = a.q + (size_t)row * a.q_stride + (size_t)head * hd;
+        for (uint32_t step = s_begin; step < s_end; ++step) {
+            const int base = (int)(start + step * S::N);
+            if (base >= any_hi || base + S::N <= any_lo) {
+                continue;
+            }
+            bool known = true, finite = true;
+            for (uint32_t i = lane; i < hd * S::N; i += 64u) {
+                const uint32_t at = (uint32_t)base + i % S::N, page = table[min(at >> shift, last_entry)];
+                known = known && page < a.cache.pages;
+                const T *v = (const T *)a.cache.v + ((size_t)(page < a.cache.pages ? page : 0u) * a.cache.kv_heads + kvh) * page_elements;
+                finite = finite && fabsf((float)v[((i / S::N) << shift) + (at & in_page)]) < INFINITY;
+            }
+            if (__all(finite) || (__all(known) && base >= all_lo && base + S::N <= all_hi)) {
+                continue;
+            }
+            for (int i = 0; i < S::N; ++i) {
+                const int at = base + i;
+                const uint32_t page = table[min((uint32_t)at >> shift, last_entry)];
+                if (page >= a.cache.pages) {
+                    continue;
+                }
+                const size_t head_page = ((size_t)page * a.cache.kv_heads + kvh) * page_elements;
+                const T *k = (const T *)a.cache.k + head_page + ((uint32_t)at & in_page) * hd;
+                const T *v = (const T *)a.cache.v + head_page + ((uint32_t)at & in_page);
+                float x = 0.0f;
+                for (uint32_t d = 0; live && d < hd; ++d) {
+                    x = fmaf(q_row[d], (float)k[d], x);
+                }
+                x = a.softcap > 0.0f ? cap_log2 * tanh_of(x * (a.scale / a.softcap)) : x * (a.scale * LOG2E);
+                x -= slope * fabsf((float)(p - at));
+                const bool seen = live && at >= lo && at < hi;
+                const float y = exp2_of(x - top + 6.0f);
+#pragma unroll
+                for (int t = 0; t < S::DT; ++t) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const uint32_t d = 32u * t + 8u * (j / 4) + 4u * h + (j % 4);
+                        o[t][j] += seen && (FULL || d < hd) ? y * (float)v[(FULL ? d : min(d, hd - 1u)) << shift] : 0.0f;
+                    }
+                }
+            }
+        }
+    }
+    l += __shfl_xor(l, 32);
+
+    // channel of value v of tile t: 32 t + 8 (v / 4) + 4 h + v % 4
+    if (parts == 1u) {
+        if (live) {
+            const float by = l == 0.0f ? 0.0f : 1.0f / l;
+            float *out = a.out + (size_t)row * a.out_stride + (size_t)head * hd;
+#pragma unroll
+            for (int t = 0; t < S::DT; ++t) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const uint32_t d = 32u * t + 8u * (v / 4) + 4u * h + (v % 4);
+                    if (FULL || d < hd) {
+                        out[d] = l == 0.0f ? 0.0f : o[t][v] * by;
+                    }
+                }
+            }
+        }
+        return;
+    }
+    // Shared positions: the parts go to memory, and the last workgroup of the tile to
+    // arrive adds them up in the order of their positions (as the decode kernel does).
+    const size_t part_floats = 128u * (size_t)(hd + 2u);
+    const size_t slot = (size_t)want * a.cache.kv_heads + kvh;
+    const float *first = args.partials + slot * args.splits * part_floats;
+    {
+        float *to = (float *)first + split * part_floats;
+        const uint32_t at = wave * 32u + c;
+        if (live) {
+#pragma unroll
+            for (int t = 0; t < S::DT; ++t) {
+#pragma unroll
+                for (int v = 0; v < 16; v += 2) {
+                    const uint32_t d = 32u * t + 8u * (v / 4) + 4u * h + (v % 4);
+                    if (FULL || d < hd) {
+                        put2(to + at * hd + d, o[t][v], o[t][v + 1]);
+                    }
+                }
+            }
+            if (h == 0u) {
+                put2(to + 128u * hd + 2u * at, top, l);
+            }
+        }
+    }
+    __builtin_amdgcn_s_waitcnt(7 << 4);
+    asm volatile("" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0u) {
+        arrived = __hip_atomic_fetch_add(&args.arrivals[slot], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (arrived != parts - 1u) {
+        return;
+    }
+    asm volatile("" ::: "memory");
+    if (threadIdx.x == 0u) {
+        __hip_atomic_store(&args.arrivals[slot], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    const uint32_t here = min(128u, rows - tile * 128u);
+    float *factor = (float *)lds; // [row][part], then 128 sums
+    float *sums = factor + 128u * PREFILL_MAX_SPLITS;
+    if (threadIdx.x < here) {
+        const float *stats = first + 128u * hd + 2u * threadIdx.x;
+        float best = -3.402823466e38f, sum = 0.0f;
+        for (uint32_t s = 0; s < parts; ++s) {
+            float t, y;
+            get2(stats + s * part_floats, t, y);
+            best = fmaxf(best, t);
+        }
+        for (uint32_t s = 0; s < parts; ++s) {
+            float t, y;
+            get2(stats + s * part_floats, t, y);
+            const float f = exp2_of(t - best);
+            factor[threadIdx.x * PREFILL_MAX_SPLITS + s] = f;
+            sum += f * y;
+        }
+        sums[threadIdx.x] = sum;
+    }
+    __syncthreads();
+    const uint32_t pairs = hd / 2u;
+    for (uint32_t i = threadIdx.x; i < here * pairs; i += 256u) {
+        const uint32_t at = i / pairs, d = 2u * (i % pairs);
+        float y0 = 0.0f, y1 = 0.0f;
+#pragma unroll 4
+        for (uint32_t s = 0; s < parts; ++s) {
+            float u0, u1;
+            get2(first + s * part_floats + at * hd + d, u0, u1);
+            const float f = factor[at * PREFILL_MAX_SPLITS + s];
+            y0 += f * u0;
+            y1 += f * u1;
+        }
+        const uint32_t rr = tile * 128u + at;
+        const float sum = sums[at];
+        float *out = a.out + (size_t)(row0 + rr / a.group) * a.out_stride + (size_t)(kvh * a.group + rr % a.group) * hd + d;
+        out[0] = sum == 0.0f ? 0.0f : y0 / sum;
+        out[1] = sum == 0.0f ? 0.0f : y1 / sum;
+    }
+}
+
+} // namespace kv

@@ -19,6 +19,35 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// tanh to a few half steps relative to its value: below 1/2 its series (the first term
+// left out is 5e-9 of it there), above it 1 - 2 t / (1 + t) with t = exp(-2 |y|),
+// which no wave computes whose values are all small (scores well below their cap).
+__device__ __forceinline__ float tanh_of(float y) {
+    const float z = y * y;
+    float s = -0.0014558344f;
+    s = fmaf(s, z, 0.0035921280f);
+    s = fmaf(s, z, -0.0088632355f);
+    s = fmaf(s, z, 0.0218694885f);
+    s = fmaf(s, z, -0.0539682540f);
+    s = fmaf(s, z, 0.1333333333f);
+    s = fmaf(s, z, -0.3333333333f);
+    float r = fmaf(y * z, s, y);
+    const bool large = !(fabsf(y) < 0.5f);
+    if (__any(large)) {
+        const float t = exp2_of(-2.0f * LOG2E * fabsf(y));
+        const float u = (1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t);
+        r = large ? copysignf(u, y) : r;
+    }
+    return r;
+}
+
+// The power of two that brings a largest magnitude to about 2^13 (none where it is not
+// finite), at which two f16 parts hold 22 bits of it without overflow.
+__device__ __forceinline__ int scale_bits(float top) {
+    const int by = top < INFINITY ? 13 - (int)((__float_as_uint(top) >> 23) & 0xffu) + 127 : 0;
+    return by < 100 ? by : 100;
+}
+
 // The value of the lane eight columns on, of sixteen.
 __device__ __forceinline__ float ror8(float x) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128, 0xf, 0xf, false));

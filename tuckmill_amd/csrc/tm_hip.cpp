@@ -2182,9 +2182,9 @@ int attention(tm_hip_ctx *ctx, const tm_hip_attn *attn, const tm_hip_kv_cache *c
         return fail(err, cap, TM_HIP_ERR_UNSUPPORTED, "%s: %u sequences (1..%u), %u rows (1..%u)", what,
                     seqs, TM_HIP_KV_MAX_SEQS, tokens, TM_HIP_KV_MAX_TOKENS);
     }
-    if (table_stride == 0 || ((uint64_t)table_stride << p.page_shift) > 0x7fffffffull) {
+    if (table_stride == 0 || ((uint64_t)table_stride << p.page_shift) > (1ull << 30)) {
         return fail(err, cap, TM_HIP_ERR_UNSUPPORTED,
-                    "%s: a table of %u pages of %u tokens per sequence (1 to 2^31 - 1 positions)", what,
+                    "%s: a table of %u pages of %u tokens per sequence (1 to 2^30 positions)", what,
                     table_stride, 1u << p.page_shift);
     }
     const uint32_t width = q_heads * p.head_dim;
@@ -2215,6 +2215,12 @@ int attention(tm_hip_ctx *ctx, const tm_hip_attn *attn, const tm_hip_kv_cache *c
     p.tokens = tokens;
     p.seqs = seqs;
     p.table_stride = table_stride;
+    const kv::AttnPlan plan = attn_plan_of(p, ragged ? OP_ATTN_PREFILL : OP_ATTN_DECODE);
+    if (ragged && plan.tile_bound * p.kv_heads * plan.splits > kv::PREFILL_MAX_GROUPS) {
+        return fail(err, cap, TM_HIP_ERR_UNSUPPORTED,
+                    "%s: %u rows of %u sequences with %u heads are more than one launch takes", what,
+                    tokens, seqs, q_heads);
+    }
     p.q_off = q_off;
     p.out_off = out_off;
     p.q_stride = q_stride;

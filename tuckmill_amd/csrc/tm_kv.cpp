@@ -3,8 +3,8 @@
 // KvParams (tm_plan.hpp) into kernel arguments, an instantiation and a grid.
 #include "tm_launch.hpp"
 
-#include "kv_attn.hpp"
 #include "kv_attn_decode.hpp"
+#include "kv_attn_prefill.hpp"
 #include "kv_logits.hpp"
 #include "kv_rope.hpp"
 
@@ -39,18 +39,6 @@ kv::AttnArgs attn_args(const Op &op) {
     return a;
 }
 
-hipError_t launch_attention(hipStream_t stream, hipEvent_t stop, const Op &op) {
-    const KvParams &p = *op.kv;
-    const kv::AttnArgs args = attn_args(op);
-    const dim3 grid(p.tokens, p.q_heads);
-    if (p.type_id == 1u) {
-        Q8_LAUNCH(kv::attn_rows_kernel<_Float16>, grid, dim3(64), 0, stream, stop, args);
-    } else {
-        Q8_LAUNCH(kv::attn_rows_kernel<float>, grid, dim3(64), 0, stream, stop, args);
-    }
-    return hipGetLastError();
-}
-
 template <typename T, int D, int W>
 hipError_t launch_decode_as(hipStream_t stream, hipEvent_t stop, const kv::DecodeArgs &args) {
     const dim3 grid(args.a.cache.kv_heads * args.head_tiles * args.splits, args.a.seqs);
@@ -78,6 +66,46 @@ hipError_t launch_decode(hipStream_t stream, hipEvent_t stop, const Op &op) {
     return d <= 64u    ? launch_decode_as<float, 64, 3>(stream, stop, args)
            : d <= 128u ? launch_decode_as<float, 128, 2>(stream, stop, args)
                        : launch_decode_as<float, 256, 1>(stream, stop, args);
+}
+
+template <typename T, int D, int W>
+hipError_t launch_prefill_as(hipStream_t stream, hipEvent_t stop, const kv::PrefillArgs &args) {
+    constexpr int LDS = 4 * kv::PrefillShape<T, D>::BYTES;
+    static_assert(LDS >= 128 * (int)(kv::PREFILL_MAX_SPLITS + 1u) * 4, "factors and sums of a join");
+    const dim3 grid(args.a.cache.kv_heads * args.splits * args.tile_bound);
+    const bool full = args.a.cache.head_dim == (uint32_t)D;
+    const void *kernel = full ? (const void *)kv::attn_prefill_kernel<T, D, true, W>
+                              : (const void *)kv::attn_prefill_kernel<T, D, false, W>;
+    if (LDS >= 65536) { // (with a few static words) beyond what a launch may ask for without saying so
+        const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        if (e != hipSuccess) {
+            return e;
+        }
+    }
+    if (full) {
+        Q8_LAUNCH((kv::attn_prefill_kernel<T, D, true, W>), grid, dim3(256), LDS, stream, stop, args);
+    } else {
+        Q8_LAUNCH((kv::attn_prefill_kernel<T, D, false, W>), grid, dim3(256), LDS, stream, stop, args);
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_prefill(hipStream_t stream, hipEvent_t stop, const Op &op) {
+    const KvParams &p = *op.kv;
+    const kv::AttnPlan plan = attn_plan_of(p, op.kind);
+    if (plan.splits > 1u && (p.partials == nullptr || p.arrivals == nullptr)) {
+        return hipErrorInvalidValue;
+    }
+    const kv::PrefillArgs args{attn_args(op), p.partials, p.arrivals, plan.splits, (uint32_t)plan.tile_bound};
+    const uint32_t d = p.head_dim;
+    if (p.type_id == 1u) {
+        return d <= 64u    ? launch_prefill_as<_Float16, 64, 2>(stream, stop, args)
+               : d <= 128u ? launch_prefill_as<_Float16, 128, 2>(stream, stop, args)
+                           : launch_prefill_as<_Float16, 256, 1>(stream, stop, args);
+    }
+    return d <= 64u    ? launch_prefill_as<float, 64, 2>(stream, stop, args)
+           : d <= 128u ? launch_prefill_as<float, 128, 2>(stream, stop, args)
+                       : launch_prefill_as<float, 256, 1>(stream, stop, args);
 }
 
 hipError_t launch_rope(hipStream_t stream, hipEvent_t stop, const Op &op) {
@@ -143,7 +171,7 @@ hipError_t tmdev::launch_kv(hipStream_t stream, hipEvent_t stop, const Op &op) {
     case OP_ATTN_DECODE:
         return launch_decode(stream, stop, op);
     case OP_ATTN_PREFILL:
-        return launch_attention(stream, stop, op);
+        return launch_prefill(stream, stop, op);
     case OP_LOGITS:
         return launch_logits(stream, stop, op);
     default:

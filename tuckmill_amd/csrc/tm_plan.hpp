@@ -103,7 +103,8 @@ inline kv::AttnPlan attn_plan_of(const KvParams &p, OpKind kind) {
         return kv::decode_plan(p.type_id, p.seqs, p.q_heads, p.kv_heads, p.head_dim,
                                (uint64_t)p.table_stride << p.page_shift);
     }
-    return kv::AttnPlan{};
+    return kv::prefill_plan(p.seqs, p.tokens, p.q_heads, p.kv_heads, p.head_dim,
+                            (uint64_t)p.table_stride << p.page_shift);
 }
 
 struct Op {
