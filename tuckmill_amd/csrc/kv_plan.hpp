@@ -64,4 +64,7 @@ inline AttnPlan prefill_plan(uint32_t seqs, uint32_t tokens, uint32_t q_heads, u
     return p;
 }
 
+// Ids of a workgroup that adjusts logits: large tiles where they still give every CU one.
+constexpr uint32_t LOGITS_LARGE = 8192, LOGITS_SMALL = 1024, LOGITS_MIN_GROUPS = 256;
+
 } // namespace kv

@@ -133,10 +133,22 @@ hipError_t launch_rope(hipStream_t stream, hipEvent_t stop, const Op &op) {
     a.rot_dim = p.rot_dim;
     a.adjacent = p.adjacent;
     memcpy(a.axis, p.axis, sizeof a.axis);
+    const dim3 grid((p.tokens + kv::ROPE_ROWS - 1u) / kv::ROPE_ROWS,
+                    (p.q_heads + p.kv_heads + kv::ROPE_HEADS - 1u) / kv::ROPE_HEADS +
+                        (p.kv_heads * p.head_dim + kv::ROPE_CHANNELS - 1u) / kv::ROPE_CHANNELS);
+    // rows and both halves of a head in 16-byte pieces (head_dim is a multiple of eight)
+    const bool wide = (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.q_out) & 15u) == 0u &&
+                      ((p.q_stride | p.k_stride | p.v_stride | p.out_stride) & 3u) == 0u && p.rot_dim % 8u == 0u;
     if (p.type_id == 1u) {
-        Q8_LAUNCH(kv::rope_store_kernel<_Float16>, dim3(p.tokens), dim3(256), 0, stream, stop, a);
+        if (wide) {
+            Q8_LAUNCH((kv::rope_store_kernel<_Float16, true>), grid, dim3(256), 0, stream, stop, a);
+        } else {
+            Q8_LAUNCH((kv::rope_store_kernel<_Float16, false>), grid, dim3(256), 0, stream, stop, a);
+        }
+    } else if (wide) {
+        Q8_LAUNCH((kv::rope_store_kernel<float, true>), grid, dim3(256), 0, stream, stop, a);
     } else {
-        Q8_LAUNCH(kv::rope_store_kernel<float>, dim3(p.tokens), dim3(256), 0, stream, stop, a);
+        Q8_LAUNCH((kv::rope_store_kernel<float, false>), grid, dim3(256), 0, stream, stop, a);
     }
     return hipGetLastError();
 }
@@ -157,8 +169,14 @@ hipError_t launch_logits(hipStream_t stream, hipEvent_t stop, const Op &op) {
     a.history_stride = p.history_stride;
     a.bias_stride = p.bias_stride;
     a.allowed_stride = p.allowed_stride;
-    const uint32_t tiles = (uint32_t)(((uint64_t)op.cols + kv::LOGITS_TILE - 1u) / kv::LOGITS_TILE);
-    Q8_LAUNCH(kv::logits_adjust_kernel, dim3(tiles, op.rows), dim3(256), 0, stream, stop, a);
+    auto tiles = [&](uint64_t tile) { return (uint32_t)((op.cols + tile - 1u) / tile); };
+    if ((uint64_t)tiles(kv::LOGITS_LARGE) * op.rows >= kv::LOGITS_MIN_GROUPS) {
+        Q8_LAUNCH((kv::logits_adjust_kernel<kv::LOGITS_LARGE, 512>), dim3(tiles(kv::LOGITS_LARGE), op.rows), dim3(512), 0,
+                  stream, stop, a);
+    } else {
+        Q8_LAUNCH((kv::logits_adjust_kernel<kv::LOGITS_SMALL, 256>), dim3(tiles(kv::LOGITS_SMALL), op.rows), dim3(256), 0,
+                  stream, stop, a);
+    }
     return hipGetLastError();
 }
 
