@@ -1,0 +1,196 @@
+"""Paged attention where a call has many rows, many sequences or long ones: ragged batches
+of f16 pages with enough rows for the kernel with tiles of 128 (more than 1024 tiles of eight
+rows over all key-value heads), and the shares that the other kernel cuts positions into."""
+import numpy as np
+import pytest
+
+import kvutil as K
+from tuckmill_amd import hip as H
+
+from q8util import require_gpu, upload_new
+from test_gpu_kv import CACHED, NEWS, f32, prefill_case, run_decode, run_prefill, want_decode, want_prefill
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = require_gpu()
+    yield c
+    c.close()
+
+
+def many(rows, seqs, heads, kv_heads):
+    """Whether the rows are enough for tiles of 128."""
+    return (rows * (heads // kv_heads) // 8 + seqs) * kv_heads > 1024
+
+
+@pytest.mark.parametrize("heads,kv_heads,d,page", [
+    (64, 64, 64, 16), (32, 16, 128, 32), (30, 10, 256, 64), (64, 64, 8, 16), (32, 32, 72, 128), (32, 16, 136, 256), (72, 12, 40, 16),
+    (32, 32, 128, 64)])
+def test_tiles_of_rows_match_the_plain_form(ctx, heads, kv_heads, d, page):
+    rng = np.random.default_rng(heads * 1000 + d + page)
+    lens = [n + c for n, c in zip(NEWS, CACHED)]
+    paged = K.Paged(rng, K.F16, page, kv_heads, d, lens)
+    starts, _, _ = prefill_case(rng, NEWS, lens)
+    assert many(int(starts[-1]) + 3, len(NEWS), heads, kv_heads)
+    q = rng.standard_normal((int(starts[-1]) + 3, heads * d)).astype(np.float32)
+    got = run_prefill(ctx, paged, q, heads, H.Attention(d ** -0.5), starts)
+    want, tol = want_prefill(paged, q, heads, starts, NEWS, np.float32(d ** -0.5))
+    K.near(got[:-3], want[:-3], tol[:-3])
+    assert (got[-3:] == 7.0).all()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("window,cap,slopes,docs,prefix,scale", [
+    (1, 0, 0, 0, 0, 1.0), (50, 5.0, 0, 0, 0, 1.0), (0, 50.0, 1, 1, 0, 1.0), (64, 0, 1, 1, 1, 1.0), (0, 0, 0, 0, 1, 1.0),
+    (0, 0, 0, 0, 0, -1.0), (0, 5.0, 1, 0, 0, -0.5), (0, 0, 0, 1, 0, 0.0)])
+def test_tiles_of_rows_with_masks_caps_and_biases(ctx, d, window, cap, slopes, docs, prefix, scale):
+    rng = np.random.default_rng(31)
+    heads = kv_heads = 32
+    lens = [n + c for n, c in zip(NEWS, CACHED)]
+    paged = K.Paged(rng, K.F16, 16, kv_heads, d, lens, scale=3.0)
+    starts, first, pre = prefill_case(rng, NEWS, lens, docs, prefix)
+    if docs:
+        first[4] = 0xffffffff  # a row that sees nothing
+    assert many(int(starts[-1]), len(NEWS), heads, kv_heads)
+    q = rng.standard_normal((int(starts[-1]), heads * d)).astype(np.float32)
+    sl = (2.0 ** -(1 + np.arange(heads) / 4)).astype(np.float32) if slopes else None
+    by = float(np.float32(d ** -0.5 * scale))
+    attn = H.Attention(by, cap, window, slopes=upload_new(ctx, sl) if slopes else None,
+                       first=upload_new(ctx, K.u32(first)) if docs else None,
+                       prefix=upload_new(ctx, K.u32(pre)) if prefix else None)
+    got = run_prefill(ctx, paged, q, heads, attn, starts)
+    want, tol = want_prefill(paged, q, heads, starts, NEWS, by, first, window, cap, sl, pre)
+    K.near(got, want, tol)
+
+
+@pytest.mark.parametrize("kv_heads,d", [(32, 64), (16, 128), (16, 256)])
+def test_tiles_of_rows_over_long_caches_share_positions(ctx, kv_heads, d):
+    rng = np.random.default_rng(32)
+    news, lens = [200, 330], [1500, 1100]
+    paged = K.Paged(rng, K.F16, 64, kv_heads, d, lens)
+    starts, _, _ = prefill_case(rng, news, lens)
+    assert many(530, 2, kv_heads, kv_heads)
+    q = rng.standard_normal((530, kv_heads * d)).astype(np.float32)
+    got = run_prefill(ctx, paged, q, kv_heads, H.Attention(d ** -0.5, window=900), starts)
+    want, tol = want_prefill(paged, q, kv_heads, starts, news, float(np.float32(d ** -0.5)), window=900)
+    K.near(got, want, tol)
+
+
+@pytest.mark.parametrize("kv_heads", [1, 64])
+@pytest.mark.parametrize("type_id", [K.F16, K.F32])
+@pytest.mark.parametrize("d", [64, 128, 256, 24])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("at", [45, 100])
+def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(ctx, kv_heads, type_id, d, bad, at):
+    rng = np.random.default_rng(33)
+    paged = K.Paged(rng, type_id, 16, kv_heads, d, [150])
+    paged.keys[0][at, 0, 3] = bad
+    paged.values[0][at] = bad
+    paged.values[0][at + 7, :, d - 2] = -bad
+    paged.put(0, at)
+    paged.put(0, at + 7)
+    q = rng.standard_normal((130, kv_heads * d)).astype(np.float32)
+    first = np.zeros(130, np.int64)
+    first[115:] = at + 8
+    attn = H.Attention(0.125, first=upload_new(ctx, K.u32(first)))
+    got = run_prefill(ctx, paged, q, kv_heads, attn, np.array([0, 130]))
+    with np.errstate(all="ignore"):
+        want, tol = want_prefill(paged, q, kv_heads, np.array([0, 130]), [130], 0.125, first)
+    p = np.arange(20, 150)
+    clean = (p < at) | (first > at + 7)
+    K.near(got[clean], want[clean], tol[clean])
+    assert np.isnan(got[clean]).sum() == 0
+    if np.isnan(bad):
+        assert np.isnan(got[~clean]).all()
+
+
+@pytest.mark.parametrize("type_id", [K.F16, K.F32])
+def test_tiles_of_rows_with_bad_pages_lengths_and_bounds(ctx, type_id):
+    rng = np.random.default_rng(34)
+    news, lens, heads = [20, 30, 10, 60], [50, 30, 10, 100], 64
+    paged = K.Paged(rng, type_id, 16, heads, 64, lens)
+    seen = [np.ones(n, bool) for n in lens]
+    paged.table[0, 1] = 0xfffffff0
+    seen[0][16:32] = False
+    paged.table[3, :] = paged.pages
+    seen[3][:] = False
+    starts, _, _ = prefill_case(rng, news, lens)
+    q = rng.standard_normal((120, heads * 64)).astype(np.float32)
+    got = run_prefill(ctx, paged, q, heads, H.Attention(0.125), starts)
+    want, tol = want_prefill(paged, q, heads, starts, news, 0.125, seen=seen)
+    K.near(got, want, tol)
+    assert not got[60:].any()
+    short = paged.lens.copy()
+    short[1] = 25
+    got = run_prefill(ctx, paged, q, heads, H.Attention(0.125), starts, short)
+    assert not got[20:25].any()
+    part, ptol = K.attention(q[25:50].reshape(25, heads, 64), paged.keys[1][:25], paged.values[1][:25], np.arange(25),
+                             *K.bounds(np.arange(25), 25), 0.125)
+    K.near(got[25:50], part, ptol)
+    got = run_prefill(ctx, paged, q, heads, H.Attention(0.125), np.array([0, 20, 10, 60, 4000000000]))
+    K.near(got[:20], want[:20], tol[:20])
+    assert (got[60:] == 7.0).all()
+
+
+def test_tiles_of_rows_at_odd_offsets_and_strides(ctx):
+    rng = np.random.default_rng(35)
+    heads, d, rows = 64, 64, 140
+    paged = K.Paged(rng, K.F16, 16, heads, d, [170])
+    w, q_off, out_off, qs, os = heads * d, 3, 5, heads * d + 7, heads * d + 2
+    q = rng.standard_normal((rows, w)).astype(np.float32)
+    flat = np.full(q_off + rows * qs, np.nan, np.float32)
+    for r in range(rows):
+        flat[q_off + r * qs:][:w] = q[r]
+    out = upload_new(ctx, np.full(out_off + rows * os + 9, 7.0, np.float32))
+    ctx.attn_prefill(H.Attention(0.125), paged.upload(ctx), upload_new(ctx, flat), upload_new(ctx, paged.table),
+                     upload_new(ctx, K.u32([170])), upload_new(ctx, K.u32([0, rows])), out, rows, 1, heads, paged.stride, q_off,
+                     out_off, qs, os)
+    ctx.fence()
+    got = f32(out, (out_off + rows * os + 9,))
+    want, tol = want_prefill(paged, q, heads, np.array([0, rows]), [rows], 0.125)
+    written = np.zeros(got.shape, bool)
+    for r in range(rows):
+        at = slice(out_off + r * os, out_off + r * os + w)
+        K.near(got[at].reshape(heads, d), want[r], tol[r])
+        written[at] = True
+    assert (got[~written] == 7.0).all()
+
+
+@pytest.mark.parametrize("type_id", [K.F16, K.F32])
+@pytest.mark.parametrize("seqs", [64, 65, 200, 513, 700])
+def test_decode_of_many_ragged_sequences(ctx, type_id, seqs):
+    rng = np.random.default_rng(seqs + type_id)
+    lens = [int(n) for n in 10 ** rng.uniform(-1, 2.3, seqs)]
+    lens[0], lens[seqs // 2], lens[-1] = 3000, 0, 2500
+    paged = K.Paged(rng, type_id, 16, 2, 64, lens)
+    q = rng.standard_normal((seqs, 4 * 64)).astype(np.float32)
+    got = run_decode(ctx, paged, q, 4, H.Attention(0.125, window=2000))
+    want, tol = want_decode(paged, q, 4, 0.125, window=2000)
+    K.near(got, want, tol)
+
+
+@pytest.mark.parametrize("type_id", [K.F16, K.F32])
+def test_ragged_rows_of_many_sequences(ctx, type_id):
+    rng = np.random.default_rng(36)
+    news = [int(n) for n in rng.integers(0, 4, 150)]
+    lens = [n + int(10 ** rng.uniform(0, 2.5)) for n in news]
+    lens[70] += 2000
+    paged = K.Paged(rng, type_id, 16, 1, 128, lens)
+    starts, _, _ = prefill_case(rng, news, lens)
+    q = rng.standard_normal((int(starts[-1]), 3 * 128)).astype(np.float32)
+    got = run_prefill(ctx, paged, q, 3, H.Attention(0.1), starts)
+    want, tol = want_prefill(paged, q, 3, starts, news, float(np.float32(0.1)))
+    K.near(got, want, tol)
+
+
+@pytest.mark.parametrize("type_id", [K.F16, K.F32])
+@pytest.mark.parametrize("scale,cap", [(-0.125, 0.0), (0.0, 0.0), (-0.5, 4.0), (0.0, 4.0)])
+def test_decode_scales_below_and_at_zero(ctx, type_id, scale, cap):
+    rng = np.random.default_rng(37)
+    paged = K.Paged(rng, type_id, 16, 2, 64, [40, 1, 333])
+    q = rng.standard_normal((3, 8 * 64)).astype(np.float32)
+    got = run_decode(ctx, paged, q, 8, H.Attention(scale, cap))
+    want, tol = want_decode(paged, q, 8, scale, softcap=cap)
+    K.near(got, want, tol)

@@ -9,38 +9,48 @@ struct DecodeArgs {
     AttnArgs a;
     float *partials;
     uint32_t *arrivals;
-    uint32_t splits, head_tiles;
+    uint32_t shares, head_tiles; // shares: to make of the positions, 0: one of each unit
 };
 
-// The matrix operands of a tile of 32 positions, in either type of page. Lane l is
-// column c = l % 16 (a query head) of group g = l / 16. The products run transposed,
+// The matrix operands of a tile of positions, in either type of page. Lane l is
+// column c = l % 16 (a row of the call) of group g = l / 16. The products run transposed,
 // S^T = K q^T and O^T = V^T P, and the positions are dealt to the rows of S^T so
-// that what a lane holds of it, positions 8 g + 0..7 for its head, is what it has
+// that what a lane holds of it, positions VALUES g + 0.. for its row, is what it has
 // to hand to the second product: the weights never leave their registers. V lies
 // in the cache with a channel's positions side by side, so both operands are read
-// from memory as they are used, 16 bytes a lane.
+// as they lie there, 16 bytes a lane. In LDS the 16-byte units of a row are swapped by
+// exclusive or with (part of) the row's number, which spreads a column of units over
+// the banks.
 // FULL: head_dim is D; else it is less, and what lies beyond it reads as zeros.
 template <typename T, int D, bool FULL> struct Tile;
 
 template <int D, bool FULL> struct Tile<_Float16, D, FULL> {
-    static constexpr int COLS = 8;        // columns 0..7 the first part of a head's q and weights, 8..15 the second
-    static constexpr int KS = D / 32;     // operand pieces of a row of K
+    static constexpr int COLS = 8;        // columns 0..7 the first part of a row's q and weights, 8..15 the second
+    static constexpr int VALUES = 8;      // of a tile of 32 positions that a lane holds
+    static constexpr int E = 8, UK = D / 8, SWIZZLE = UK < 16 ? UK - 1 : 15; // 16-byte units: elements, of a key
+    static constexpr int KS = D / 32;     // operand pieces of a key
     static constexpr int DT = D / 16;     // channel tiles
+    static constexpr int HALVES = 2;      // of 16 keys each in a tile's stage
+    static constexpr bool PARTS = true;
     typedef f16x8 K[2][KS];
     typedef f16x8 V[DT];
+    typedef f32x4 S[2];
     f16x8 q[KS];
 
-    // The head's q, scaled by a power of two to a largest magnitude of about 2^13, as
+    // The row's q, scaled by a power of two to a largest magnitude of about 2^13, as
     // f16 parts (22 bits of that magnitude); returns the inverse scale. What is
     // not finite goes whole into the first part.
-    __device__ __forceinline__ float load_q(const float *row, uint32_t c, uint32_t g, uint32_t hd, bool live) {
+    __device__ __forceinline__ float load_q(const float *row, uint32_t c, uint32_t g, uint32_t hd, bool live, float sign) {
         float x[KS][8], top = 0.0f;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
+            const uint32_t d = 32u * s + 8u * g;
+            const bool there = live && (FULL || d < hd);
+            const float *from = row + (FULL || d < hd ? d : 0u);
+            const f32x4 y[2] = {*(const f32x4_unaligned *)from, *(const f32x4_unaligned *)(from + 4)};
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const uint32_t d = 32u * s + 8u * g + j;
-                x[s][j] = live && d < hd ? row[d] : 0.0f;
+                x[s][j] = there ? y[j / 4][j % 4] : 0.0f;
                 top = fmaxf(top, fabsf(x[s][j]));
             }
         }
@@ -51,7 +61,7 @@ template <int D, bool FULL> struct Tile<_Float16, D, FULL> {
         for (int s = 0; s < KS; ++s) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float y = ldexpf(x[s][j], by);
+                const float y = ldexpf(x[s][j] * sign, by);
                 const _Float16 hi = (_Float16)y;
                 const float rest = fabsf((float)hi) < INFINITY ? y - (float)hi : 0.0f;
                 q[s][j] = c < 8u ? hi : (_Float16)rest;
@@ -59,145 +69,222 @@ template <int D, bool FULL> struct Tile<_Float16, D, FULL> {
         }
         return ldexpf(1.0f, -by);
     }
-    // K row of lane l in half t of the tile: position 8 (r / 4) + r % 4 + 4 t for r = l % 16
-    __device__ __forceinline__ void load_k(K &k, const _Float16 *row0, uint32_t g, uint32_t hd) const {
+    // row `at` of a stage of keys (16 a half) is this position of the tile
+    static constexpr __device__ __forceinline__ uint32_t k_position(uint32_t at) {
+        return 8u * ((at & 15u) >> 2) + (at & 3u) + 4u * (at >> 4);
+    }
+    __device__ __forceinline__ void read_k(K &k, const uint8_t *stage, uint32_t c, uint32_t g, uint32_t hd) const {
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            const uint32_t d = 32u * s + 8u * g;
-            const bool in = FULL || d < hd;
+            const uint32_t unit = 4u * s + g;
+            const bool in = FULL || 8u * unit < hd;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const f16x8 x = *(const f16x8 *)(row0 + 4u * t * (FULL ? D : hd) + (in ? d : 0u));
+                const uint32_t at = 16u * t + c;
+                const f16x8 x = *(const f16x8 *)(stage + (at * UK + (unit ^ (at & SWIZZLE))) * 16u);
                 k[t][s] = in ? x : f16x8{};
             }
         }
     }
     // channel 16 t + c, positions 8 g + 0..7
-    __device__ __forceinline__ void load_v(V &v, const _Float16 *at, uint32_t c, uint32_t shift, uint32_t hd) const {
+    __device__ __forceinline__ void read_v(V &v, const uint8_t *stage, uint32_t c, uint32_t g) const {
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
-            const uint32_t d = 16u * t + c; // (results of channels beyond the last are not used)
-            v[t] = *(const f16x8 *)(at + ((FULL ? d : min(d, hd - 1u)) << shift));
+            const uint32_t d = 16u * t + c;
+            v[t] = *(const f16x8 *)(stage + (d * 4u + (g ^ ((d >> 2) & 3u))) * 16u);
         }
     }
-    __device__ __forceinline__ void scores(float (&x)[8], const K &k, uint32_t c) const {
+    __device__ __forceinline__ void products(S &acc, const K &k) const {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+            acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][s], q[s], acc, 0, 0, 0);
-            }
+        for (int s = 0; s < KS; ++s) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                // both parts of the head: columns c and c + 8 of 16. Where the key is infinite the
-                // first part's infinity (or NaN) is the score, whatever the second one gives.
-                const float part = c < 8u ? acc[i] : __builtin_amdgcn_fmed3f(acc[i], -3.402823466e38f, 3.402823466e38f);
-                x[4 * t + i] = part + ror8(part);
+            for (int t = 0; t < 2; ++t) {
+                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][s], q[s], acc[t], 0, 0, 0);
             }
         }
     }
-    __device__ __forceinline__ void weigh(f32x4 (&o)[DT], const V &v, const float (&w)[8], uint32_t c) const {
+    // Both parts of the row: columns c and c + 8 of 16. Where a key is infinite the first
+    // part's infinity (or NaN) is the score, whatever the second one gives: `careful`.
+    static __device__ __forceinline__ void scores(float (&x)[VALUES], const S &acc, uint32_t c, bool careful) {
+#pragma unroll
+        for (int j = 0; j < VALUES; ++j) {
+            const float y = acc[j / 4][j % 4];
+            const float part = careful && c >= 8u ? __builtin_amdgcn_fmed3f(y, -3.402823466e38f, 3.402823466e38f) : y;
+            x[j] = part + ror8(part);
+        }
+    }
+    // the part of the weights that the column stands for
+    static __device__ __forceinline__ f16x8 part_of(const float (&w)[VALUES], uint32_t c) {
+        const float second = c < 8u ? 0.0f : -1.0f;
         f16x8 p;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const _Float16 hi = (_Float16)w[j];
-            p[j] = c < 8u ? hi : (_Float16)(w[j] - (float)hi);
+        for (int j = 0; j < VALUES; ++j) {
+            p[j] = (_Float16)fmaf((float)(_Float16)w[j], second, w[j]);
         }
+        return p;
+    }
+    __device__ __forceinline__ void weigh(f32x4 (&o)[DT], const V &v, const float (&w)[VALUES], uint32_t c) const {
+        const f16x8 p = part_of(w, c);
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
             o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], p, o[t], 0, 0, 0);
         }
     }
+    // weigh() where values that are not finite meet rows that do not see them (part_finite):
+    // a row sees the lane's positions from <= j < upto.
+    __device__ __forceinline__ void weigh_finite(f32x4 (&o)[DT], const V &v, const float (&w)[VALUES], uint32_t c, int from,
+                                                 int upto) const {
+        const f16x8 p = part_of(w, c);
+        f16x8 ones;
+#pragma unroll
+        for (int j = 0; j < VALUES; ++j) {
+            ones[j] = (_Float16)(j >= from && j < upto ? 1.0f : 0.0f);
+        }
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+            f16x8 clean = v[t], wrong;
+            part_finite<_Float16, f16x8, 8>(clean, wrong);
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(clean, p, o[t], 0, 0, 0);
+            f32x4 count = {0.0f, 0.0f, 0.0f, 0.0f};
+            count = __builtin_amdgcn_mfma_f32_16x16x32_f16(wrong, ones, count, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                o[t][i] = count[i] > 0.0f ? NAN : o[t][i];
+            }
+        }
+    }
     // positions whose bit of `mask` is not set as zeros (0 x infinity would be NaN)
-    __device__ __forceinline__ void clear(V &v, uint32_t mask) const {
+    static __device__ __forceinline__ void clear(V &v, uint32_t mask) {
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < VALUES; ++j) {
                 v[t][j] = (mask >> j) & 1u ? v[t][j] : (_Float16)0.0f;
             }
         }
     }
-    __device__ __forceinline__ float whole(float x) const { return x + ror8(x); }
+    static __device__ __forceinline__ bool finite(const V &v) {
+        float bad = 0.0f;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+#pragma unroll
+            for (int j = 0; j < VALUES; ++j) {
+                bad += 0.0f * (float)v[t][j];
+            }
+        }
+        return bad == 0.0f;
+    }
+    static __device__ __forceinline__ float whole(float x) { return x + ror8(x); }
 };
 
 template <int D, bool FULL> struct Tile<float, D, FULL> {
     static constexpr int COLS = 16;
+    static constexpr int VALUES = 4; // of a tile of 16 positions
+    static constexpr int E = 4, UK = D / 4, SWIZZLE = 15;
     static constexpr int KS = D / 16;
     static constexpr int DT = D / 16;
-    typedef f32x4 K[2][KS];
-    typedef f32x4 V[DT][2];
+    static constexpr int HALVES = 1;
+    static constexpr bool PARTS = false;
+    typedef f32x4 K[KS];
+    typedef f32x4 V[DT];
+    typedef f32x4 S;
     f32x4 q[KS];
 
-    __device__ __forceinline__ float load_q(const float *row, uint32_t, uint32_t g, uint32_t hd, bool live) {
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t d = 16u * s + 4u * g + j;
-                q[s][j] = live && d < hd ? row[d] : 0.0f;
-            }
-        }
-        return 1.0f;
-    }
-    __device__ __forceinline__ void load_k(K &k, const float *row0, uint32_t g, uint32_t hd) const {
+    __device__ __forceinline__ float load_q(const float *row, uint32_t, uint32_t g, uint32_t hd, bool live, float sign) {
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const uint32_t d = 16u * s + 4u * g;
-            const bool in = FULL || d < hd;
+            const f32x4 x = *(const f32x4_unaligned *)(row + (FULL || d < hd ? d : 0u)) * sign;
+            q[s] = live && (FULL || d < hd) ? x : f32x4{};
+        }
+        return 1.0f;
+    }
+    static constexpr __device__ __forceinline__ uint32_t k_position(uint32_t at) { return at; }
+    __device__ __forceinline__ void read_k(K &k, const uint8_t *stage, uint32_t c, uint32_t g, uint32_t hd) const {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const f32x4 x = *(const f32x4 *)(row0 + 4u * t * (FULL ? D : hd) + (in ? d : 0u));
-                k[t][s] = in ? x : f32x4{};
-            }
+        for (int s = 0; s < KS; ++s) {
+            const uint32_t unit = 4u * s + g;
+            const f32x4 x = *(const f32x4 *)(stage + (c * UK + (unit ^ (c & SWIZZLE))) * 16u);
+            k[s] = FULL || 4u * unit < hd ? x : f32x4{};
         }
     }
-    __device__ __forceinline__ void load_v(V &v, const float *at, uint32_t c, uint32_t shift, uint32_t hd) const {
+    __device__ __forceinline__ void read_v(V &v, const uint8_t *stage, uint32_t c, uint32_t g) const {
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
             const uint32_t d = 16u * t + c;
-            const float *p = at + ((FULL ? d : min(d, hd - 1u)) << shift);
-            v[t][0] = *(const f32x4 *)p;
-            v[t][1] = *(const f32x4 *)(p + 4);
+            v[t] = *(const f32x4 *)(stage + (d * 4u + (g ^ ((d >> 2) & 3u))) * 16u);
         }
     }
-    __device__ __forceinline__ void scores(float (&x)[8], const K &k, uint32_t) const {
+    __device__ __forceinline__ void products(S &acc, const K &k) const {
+        // (two sums: a product waits for the one before it in its sum)
+        f32x4 even = {0.0f, 0.0f, 0.0f, 0.0f}, odd = even;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int s = 0; s < KS; ++s) {
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
+            for (int j = 0; j < 4; j += 2) {
+                even = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][j], q[s][j], even, 0, 0, 0);
+                odd = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][j + 1], q[s][j + 1], odd, 0, 0, 0);
+            }
+        }
+        acc = even + odd;
+    }
+    static __device__ __forceinline__ void scores(float (&x)[VALUES], const S &acc, uint32_t, bool) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][s][j], q[s][j], acc, 0, 0, 0);
-                }
+        for (int j = 0; j < VALUES; ++j) {
+            x[j] = acc[j];
+        }
+    }
+    __device__ __forceinline__ void weigh(f32x4 (&o)[DT], const V &v, const float (&w)[VALUES], uint32_t) const {
+#pragma unroll
+        for (int j = 0; j < VALUES; ++j) {
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+                o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[t][j], w[j], o[t], 0, 0, 0);
+            }
+        }
+    }
+    __device__ __forceinline__ void weigh_finite(f32x4 (&o)[DT], const V &v, const float (&w)[VALUES], uint32_t, int from,
+                                                 int upto) const {
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+            f32x4 clean = v[t], wrong, count = {0.0f, 0.0f, 0.0f, 0.0f};
+            part_finite<float, f32x4, 4>(clean, wrong);
+#pragma unroll
+            for (int j = 0; j < VALUES; ++j) {
+                o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(clean[j], w[j], o[t], 0, 0, 0);
+                count = __builtin_amdgcn_mfma_f32_16x16x4f32(wrong[j], j >= from && j < upto ? 1.0f : 0.0f, count, 0, 0, 0);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                x[4 * t + i] = acc[i];
+                o[t][i] = count[i] > 0.0f ? NAN : o[t][i];
             }
         }
     }
-    __device__ __forceinline__ void weigh(f32x4 (&o)[DT], const V &v, const float (&w)[8], uint32_t) const {
+    static __device__ __forceinline__ void clear(V &v, uint32_t mask) {
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[t][j / 4][j % 4], w[j], o[t], 0, 0, 0);
+            for (int j = 0; j < VALUES; ++j) {
+                v[t][j] = (mask >> j) & 1u ? v[t][j] : 0.0f;
             }
         }
     }
-    __device__ __forceinline__ void clear(V &v, uint32_t mask) const {
+    static __device__ __forceinline__ bool finite(const V &v) {
+        float bad = 0.0f;
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[t][j / 4][j % 4] = (mask >> j) & 1u ? v[t][j / 4][j % 4] : 0.0f;
+            for (int j = 0; j < VALUES; ++j) {
+                bad += 0.0f * v[t][j];
             }
         }
+        return bad == 0.0f;
     }
-    __device__ __forceinline__ float whole(float x) const { return x; }
+    static __device__ __forceinline__ float whole(float x) { return x; }
 };
 
 // Partial results of the workgroups that share a sequence travel in 8-byte
@@ -212,131 +299,378 @@ __device__ __forceinline__ void get2(const float *at, float &x, float &y) {
     y = __uint_as_float((uint32_t)(v >> 32));
 }
 
-// A workgroup of four waves per key-value head, tile of its query heads, sequence
-// and share of the positions; a wave takes every fourth tile of 32 positions
-// straight from memory into the matrix operands. The softmax runs over one pass:
-// weights are 2^(x - m + 6) with a reference m per head that follows the maximum
-// only when that has moved by more than 8 (so weights stay below 2^14, exact in two
-// f16 parts, and most tiles need no exchange between lanes); l and o are
-// their f32 sums. The waves join in LDS, the workgroups of a sequence through
-// memory: the last to arrive adds the parts up in the order of their positions.
-template <typename T, int D, bool FULL, int WAVES_PER_SIMD>
-__global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_decode_kernel(DecodeArgs args) {
+// 64 x 16 bytes from memory into 1 KiB of LDS: from the lanes' addresses, or from 32-bit
+// offsets beyond a common one. From inline assembly, and waited for by hand: the
+// compiler's own bookkeeping would order every LDS read behind all such loads in flight.
+__device__ __forceinline__ void fetch16(const void *from, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(from) : "memory", "m0");
+}
+__device__ __forceinline__ void fetch16(const void *base, uint32_t offset, uint32_t lds) {
+    const uint64_t at = (uint64_t)(uintptr_t)base; // (the same in every lane; said, not left to be found out)
+    const uint32_t low = __builtin_amdgcn_readfirstlane((uint32_t)at); // (an int until it is an unsigned one)
+    const uint32_t high = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
+    const uint64_t uniform = (uint64_t)high << 32 | low;
+    // (five wait states between a vector instruction that writes a scalar register and the
+    // memory instruction that reads it: here the compiler does not see the latter)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(lds), "v"(offset), "s"(uniform)
+                 : "memory", "m0");
+}
+// past this die's L2, as get2
+__device__ __forceinline__ void fetch16_past(const void *from, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off sc1" : : "s"(lds), "v"(from) : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t lds_address(const uint8_t *p) {
+    return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)p);
+}
+
+// Waits until at most N of the wave's fetches are in flight; its reads of LDS are done.
+template <int N> __device__ __forceinline__ void wait_fetches() {
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4));
+    asm volatile("" ::: "memory");
+}
+
+// A unit of work is a key-value head and a tile of rows; a row is a query and a head of
+// the key-value head's group (RAGGED: the rows of tm_hip_attn_prefill where a sequence
+// has few, else one query a sequence). The positions of all units, in steps of a tile for
+// each of the four waves, are cut into shares of nearly one size, as many as keep the card
+// busy: sequences of any lengths end together. A share lies in one unit (one that ran
+// on into the next unit would save 1% of the steps and cost a second prologue and join).
+// The keys and values of a tile of positions come straight from the pages into the wave's
+// own LDS; each half (keys, then values) is fetched again as soon as it has been
+// read, so that one of the two is always on its way, the waves never wait for
+// each other before the end, and registers do not bound what is in flight. A fetch
+// costs no vector instruction: the lanes' offsets stay the same from tile to
+// tile, pages and places move the scalar base.
+// The softmax runs over one pass: weights are 2^(x - m + 6) with a reference m
+// per row that follows the maximum only when that has moved by more than 8 (so weights
+// stay below 2^14, exact in two f16 parts, and most tiles need no exchange between
+// lanes); l and o are their f32 sums. The waves join in LDS, the workgroups of a
+// unit through memory: the last to arrive adds the parts up in the order of
+// their positions.
+// Bound by memory where queries are few: one sequence of 131071 tokens, 8 heads of 128
+// channels in f16, 100 us = 5.4 TB/s; 777 tokens 9 us, of which the launch is most. Short calls
+// are bound by the way through the code, every line of which is fetched once: loads of q in
+// wide pieces and a rolled join (20 KB of code for 30) took 16 sequences in f32 from 57 to 30 us.
+template <typename T, int D, bool FULL, bool RAGGED>
+__global__ __launch_bounds__(64 * DECODE_WAVES, D <= 128 ? 2 : 1) void attn_decode_kernel(DecodeArgs args) {
     typedef Tile<T, D, FULL> M;
-    constexpr int COLS = M::COLS, DT = M::DT, PITCH = D + 4;
-    __shared__ __align__(16) float merged[4 * COLS * PITCH];
-    __shared__ float stats[4][2][COLS];
+    constexpr int COLS = M::COLS, DT = M::DT, PITCH = D + 4, VALUES = M::VALUES, TOKENS = 4 * VALUES;
+    constexpr int NW = DECODE_WAVES, THREADS = 64 * NW;
+    constexpr int BYTES = TOKENS * D * (int)sizeof(T), FETCHES = BYTES / 1024; // keys or values of a tile
+    constexpr int PAGES = TOKENS / 16, KINDS = FETCHES / M::HALVES; // of lane offsets of keys
+    constexpr int PARTS = D <= 64 ? 16 : 32; // that a join takes at a time, of 2 KiB at most
+    extern __shared__ __align__(16) uint8_t lds[]; // keys and values of each wave; at the end the waves' results
+    static_assert(COLS * PITCH * 4 <= 2 * BYTES && PARTS * 2048 <= NW * 2 * BYTES && 8 * THREADS <= 2048, "results");
+    float *merged = (float *)lds;
+    __shared__ float stats[NW][2][COLS];
+    __shared__ float joins[PARTS][COLS][2];
     __shared__ uint32_t arrived;
     const AttnArgs &a = args.a;
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t c = lane & 15u, g = lane >> 4;
-    const uint32_t units = a.cache.kv_heads * args.head_tiles;
-    const uint32_t seq = blockIdx.y, split = blockIdx.x / units, unit = blockIdx.x % units;
-    const uint32_t kvh = unit % a.cache.kv_heads, head_tile = unit / a.cache.kv_heads;
     const uint32_t hd = FULL ? (uint32_t)D : a.cache.head_dim, shift = a.cache.page_shift;
-    const uint32_t heads = min((uint32_t)COLS, a.group - head_tile * COLS); // of this tile
-    const uint32_t head0 = kvh * a.group + head_tile * COLS;
-
-    const int len = seq_len(a, seq), p = len - 1;
-    int lo, hi;
-    visible(a, len, seq, seq, p, lo, hi);
-    const int start = lo & ~31;
-    const uint32_t tiles = hi > lo ? (uint32_t)(hi - start + 31) >> 5 : 0u;
-    const uint32_t per = (((tiles + args.splits - 1u) / args.splits) + 3u) & ~3u;
-    const uint32_t parts = tiles > per ? (tiles + per - 1u) / per : 1u;
-    if (split >= parts) {
-        return;
+    const size_t part_floats = (size_t)COLS * (hd + 2u);
+    const uint32_t last_entry = a.table_stride - 1u, in_page = (1u << shift) - 1u;
+    const uint32_t page_elements = hd << shift;
+    const uint8_t *stage = lds + wave * (2u * BYTES);
+    const uint32_t k_lds = lds_address(stage), v_lds = k_lds + BYTES;
+    // A fetch of keys is rows 64 / UK of the stage, all within 16 positions of the tile.
+    constexpr uint32_t ROWS = 64u / M::UK;
+    uint32_t k_offset[KINDS];
+#pragma unroll
+    for (int f = 0; f < KINDS; ++f) {
+        const uint32_t at = f * ROWS + lane / M::UK, d = ((lane % M::UK) ^ (at & M::SWIZZLE)) * M::E;
+        k_offset[f] = ((M::k_position(at) & 15u) * hd + (FULL || d < hd ? d : 0u)) * (uint32_t)sizeof(T);
     }
-    const uint32_t t1 = min(tiles, (split + 1u) * per);
+    // A fetch of values is 16 channels' units of the tile.
+    const uint32_t v_row = lane >> 2, v_position = ((lane & 3u) ^ ((v_row >> 2) & 3u)) * M::E;
+
+    // What there is to do, and this workgroup's share of it.
+    auto units_of = [&](uint32_t s, uint32_t n) { // of a sequence of n rows
+        return RAGGED ? (n * a.group + COLS - 1u) / COLS * a.cache.kv_heads : a.cache.kv_heads * args.head_tiles;
+    };
+    // Steps of a unit: of the positions that the sequence's query sees, or (RAGGED, where
+    // every row sees its own) all that any could.
+    auto steps_of = [&](uint32_t s, uint32_t n) {
+        const int len = seq_len(a, s);
+        int lo = 0, hi = len;
+        if constexpr (!RAGGED) {
+            visible(a, len, s, s, len - 1, lo, hi);
+        } else if (a.window != 0u && a.prefix == nullptr) {
+            hi = (int)min((uint64_t)len, (uint64_t)a.window + n + TOKENS);
+        }
+        const uint32_t tiles = lo < hi ? ((uint32_t)hi - ((uint32_t)lo & ~(uint32_t)(TOKENS - 1)) + TOKENS - 1u) / TOKENS : 0u;
+        return max(1u, (tiles + NW - 1u) / NW); // (a unit that sees nothing has zeros to write)
+    };
+    uint32_t seq = blockIdx.y, tile = blockIdx.x / a.cache.kv_heads, kvh = blockIdx.x % a.cache.kv_heads;
+    uint32_t row0 = seq, rows = a.group, part = 0, parts = 1, slot = 0;
+    if (RAGGED || args.shares != 0u) {
+        // 64 sequences, one a lane: its rows, a unit's steps, and the sum up to its end: of steps, or
+        // (once the size of a share is known) of shares, and in the high half of those that
+        // are not all of their unit
+        uint32_t s0 = 0, highest = 0, rows_up_to = 0, rows_here = 0, steps_here = 0, size = 0;
+        uint64_t before = 0, upto = 0; // `before`: of the sequences before s0
+        auto look = [&]() {
+            rows_up_to = highest;
+            const uint32_t s = min(s0 + lane, a.seqs - 1u);
+            rows_here = RAGGED ? rows_of(a, s0, rows_up_to) : s0 + lane < a.seqs ? 1u : 0u;
+            steps_here = rows_here != 0u ? steps_of(s, rows_here) : 0u;
+            const uint64_t shares = size != 0u ? (steps_here + size - 1u) / size : 0u;
+            upto = (uint64_t)units_of(s, rows_here) * (size == 0u ? steps_here : shares > 1u ? shares | shares << 32 : shares);
+            for (uint32_t x = 1; x < 64u; x <<= 1) {
+                const uint64_t y = __shfl_up(upto, x);
+                upto += lane >= x ? y : 0u;
+            }
+        };
+        auto look_on = [&]() {
+            before += __shfl(upto, 63);
+            highest = rows_up_to;
+            s0 += 64u;
+            look();
+        };
+        look();
+        while (s0 + 64u < a.seqs) {
+            look_on();
+        }
+        size = (uint32_t)((before + __shfl(upto, 63) + args.shares - 1u) / args.shares);
+        size = __builtin_amdgcn_readfirstlane(max(size, 1u));
+        s0 = highest = 0;
+        before = 0;
+        look();
+        uint64_t found;
+        while ((found = __ballot(blockIdx.x < (uint32_t)(before + upto))) == 0ull) {
+            if (s0 + 64u >= a.seqs) {
+                return;
+            }
+            look_on();
+        }
+        const int at = __builtin_ctzll(found);
+        seq = s0 + (uint32_t)at;
+        parts = (__shfl(steps_here, at) + size - 1u) / size;
+        rows = __shfl(rows_here, at) * a.group;
+        row0 = RAGGED ? a.starts[seq] : seq;
+        before += at > 0 ? __shfl(upto, at - 1) : 0u;
+        const uint32_t index = blockIdx.x - (uint32_t)before, unit = index / parts;
+        part = index % parts;
+        slot = (uint32_t)(before >> 32) + unit * parts; // (at most two for each full share)
+        kvh = unit % a.cache.kv_heads;
+        tile = unit / a.cache.kv_heads;
+        seq = __builtin_amdgcn_readfirstlane(seq);
+        parts = __builtin_amdgcn_readfirstlane(parts);
+        part = __builtin_amdgcn_readfirstlane(part);
+        tile = __builtin_amdgcn_readfirstlane(tile);
+        kvh = __builtin_amdgcn_readfirstlane(kvh);
+        row0 = __builtin_amdgcn_readfirstlane(row0);
+        rows = __builtin_amdgcn_readfirstlane(rows);
+        slot = __builtin_amdgcn_readfirstlane(slot); // of the unit's first part
+    }
+    const uint32_t first_row = tile * COLS, here = min((uint32_t)COLS, rows - first_row); // of this tile
+
+    // this lane's row, what it sees, what any row of the tile sees and what all see
+    const uint32_t col = COLS == 8 ? c & 7u : c;
+    const bool live = col < here;
+    const uint32_t r = first_row + (live ? col : 0u);
+    const uint32_t query = RAGGED ? r / a.group : 0u, head = kvh * a.group + (RAGGED ? r % a.group : r);
+    const int len = seq_len(a, seq);
+    const int p = RAGGED ? len - (int)(rows / a.group) + (int)query : len - 1;
+    int lo, hi;
+    visible(a, len, seq, row0 + query, p, lo, hi);
+    int any_lo = lo < hi ? lo : 0x7fffffff, any_hi = lo < hi ? hi : 0, all_lo = lo, all_hi = hi;
+    if constexpr (RAGGED) {
+        for (int x = 8; x > 0; x >>= 1) {
+            any_lo = min(any_lo, __shfl_xor(any_lo, x));
+            any_hi = max(any_hi, __shfl_xor(any_hi, x));
+            all_lo = max(all_lo, __shfl_xor(all_lo, x));
+            all_hi = min(all_hi, __shfl_xor(all_hi, x));
+        }
+    }
+    any_lo = __builtin_amdgcn_readfirstlane(any_lo);
+    any_hi = __builtin_amdgcn_readfirstlane(any_hi);
+    all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+    all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+    const uint32_t start = any_lo < any_hi ? (uint32_t)any_lo & ~(uint32_t)(TOKENS - 1) : 0u;
+    const uint32_t tiles = any_lo < any_hi ? ((uint32_t)any_hi - start + TOKENS - 1u) / TOKENS : 0u;
+    const uint32_t each = (tiles + parts * NW - 1u) / (parts * NW); // of a wave
+    const uint32_t t0 = min(tiles, (part * NW + wave) * each), n = min(tiles, t0 + each) - t0;
+
+    // Pages of a tile, one for every 16 positions, looked up ahead.
+    const __attribute__((address_space(4))) uint32_t *table =
+        (const __attribute__((address_space(4))) uint32_t *)(a.table + (size_t)seq * a.table_stride);
+    struct Pages {
+        uint32_t id[PAGES];
+    };
+    auto look_up = [&](uint32_t i) {
+        Pages p;
+        const uint32_t base = start + TOKENS * (t0 + i);
+#pragma unroll
+        for (int b = 0; b < PAGES; ++b) {
+            p.id[b] = table[min((base + 16u * b) >> shift, last_entry)];
+        }
+        return p;
+    };
+    auto head_page = [&](uint32_t page) { // (a page that is not there is not seen: somewhere to read from)
+        return ((size_t)(page < a.cache.pages ? page : 0u) * a.cache.kv_heads + kvh) * page_elements;
+    };
+    auto fetch_k = [&](uint32_t i, const Pages &p) {
+        const uint32_t base = start + TOKENS * (t0 + i);
+#pragma unroll
+        for (int b = 0; b < PAGES; ++b) {
+            const uint8_t *page = (const uint8_t *)((const T *)a.cache.k + head_page(p.id[b]) + ((base + 16u * b) & in_page) * hd);
+#pragma unroll
+            for (int f = 0; f < FETCHES; ++f) {
+                if ((int)(M::k_position(f * ROWS) >> 4) == b) {
+                    // (the second half of a stage lies four positions on)
+                    fetch16(page + (f / KINDS) * (4u * hd * sizeof(T)), k_offset[f % KINDS], k_lds + f * 1024);
+                }
+            }
+        }
+    };
+    auto fetch_v = [&](uint32_t i, const Pages &p) {
+        const uint32_t base = start + TOKENS * (t0 + i);
+        const T *v = (const T *)a.cache.v + head_page(p.id[0]) + (base & in_page);
+        if (PAGES == 1 || in_page >= (uint32_t)TOKENS - 1u) {
+#pragma unroll
+            for (int f = 0; f < FETCHES; ++f) { // (channels beyond the last: results that are not used)
+                const uint32_t d = FULL ? v_row : min(16u * f + v_row, hd - 1u);
+                fetch16(v + (FULL ? (16u * f) << shift : 0u), ((d << shift) + v_position) * (uint32_t)sizeof(T), v_lds + f * 1024);
+            }
+        } else { // pages of 16 positions
+            const T *second = (const T *)a.cache.v + head_page(p.id[PAGES - 1]);
+            const T *mine = (v_position < 16u ? v : second) + (v_position & 15u);
+#pragma unroll
+            for (int f = 0; f < FETCHES; ++f) {
+                fetch16(mine + ((FULL ? 16u * f + v_row : min(16u * f + v_row, hd - 1u)) << shift), v_lds + f * 1024);
+            }
+        }
+    };
+    Pages now = {}, next = {};
+    if (n > 0u) {
+        now = look_up(0u);
+        fetch_k(0u, now);
+        fetch_v(0u, now);
+        next = look_up(1u);
+    }
 
     M m;
-    const uint32_t col = COLS == 8 ? c & 7u : c;
-    const bool live = col < heads;
-    const float unscale = m.load_q(a.q + (size_t)seq * a.q_stride + (size_t)(head0 + (live ? col : 0u)) * hd, c, g, hd, live);
-    const float slope = a.slopes != nullptr && live ? a.slopes[head0 + col] * LOG2E : 0.0f;
-    const float to_log2 = a.softcap > 0.0f ? a.scale * unscale / a.softcap : a.scale * unscale * LOG2E;
+    const float unscale = m.load_q(a.q + (size_t)(row0 + query) * a.q_stride + (size_t)head * hd, c, g, hd, live,
+                                   a.scale < 0.0f ? -1.0f : 1.0f);
+    const float slope = a.slopes != nullptr ? a.slopes[head] * LOG2E : 0.0f;
+    const float scale = fabsf(a.scale) * unscale; // (its sign is with q)
+    const float to_log2 = a.softcap > 0.0f ? scale / a.softcap : scale * LOG2E;
     const float cap_log2 = a.softcap * LOG2E;
 
     f32x4 o[DT];
 #pragma unroll
-    for (int t = 0; t < DT; ++t) {
-        o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < DT; ++i) {
+        o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     float top = -3.402823466e38f, l = 0.0f;
 
-    const uint32_t *table = a.table + (size_t)seq * a.table_stride;
-    const uint32_t last_entry = a.table_stride - 1u, in_page = (1u << shift) - 1u;
-    const uint32_t page_elements = hd << shift;
-    auto head_page = [&](uint32_t page) { return ((size_t)page * a.cache.kv_heads + kvh) * page_elements; };
-    const uint32_t row = 8u * (c >> 2) + (c & 3u); // of K in the tile's first half
-    for (uint32_t t = split * per + wave; t < t1; t += 4u) {
-        const uint32_t base = (uint32_t)start + 32u * t;
-        const uint32_t k_page = table[min((base + row) >> shift, last_entry)];
-        const uint32_t v_page = table[min((base + 8u * g) >> shift, last_entry)];
-        const bool known = v_page < a.cache.pages;
-        typename M::K k;
-        typename M::V v;
-        const size_t k_at = head_page(k_page < a.cache.pages ? k_page : 0u);
-        const size_t v_at = head_page(known ? v_page : 0u);
-        m.load_k(k, (const T *)a.cache.k + k_at + ((base + row) & in_page) * hd, g, hd);
-        m.load_v(v, (const T *)a.cache.v + v_at + ((base + 8u * g) & in_page), c, shift, hd);
-        float x[8];
-        m.scores(x, k, c);
-        if (a.softcap > 0.0f) {
+    for (uint32_t i = 0; i < n; ++i) {
+        const uint32_t base = start + TOKENS * (t0 + i);
+        const Pages after = look_up(i + 2u);
+        typename M::S acc;
+        {
+            wait_fetches<FETCHES>(); // all but this tile's values
+            typename M::K k;
+            m.read_k(k, stage, c, g, hd);
+            m.products(acc, k);
+        }
+        if (i + 1u < n) {
+            wait_fetches<FETCHES>(); // (the reads of the keys)
+            fetch_k(i + 1u, next);
+        }
+        const bool known = (PAGES == 1 || g < 2u ? now.id[0] : now.id[PAGES - 1]) < a.cache.pages;
+        const int at = (int)(base + VALUES * g);
+        const bool whole = __all((int)base >= all_lo && (int)base + TOKENS <= all_hi && known);
+        uint32_t mask = 0;
+        float w[VALUES];
+        float keep = 1.0f, sum = l;
+        for (bool careful = false;; careful = true) {
+            float x[VALUES];
+            M::scores(x, acc, c, careful);
+            // (rounded before the reference is taken from it: a fused difference would leave
+            // a huge score's rounding in the exponent)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[j] = cap_log2 * tanh_of(x[j] * to_log2);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < VALUES; ++j) {
                 x[j] *= to_log2;
             }
-        }
-        const int at = (int)(base + 8u * g);
-        if (a.slopes != nullptr) {
+            if (a.softcap > 0.0f) {
+                cap_of(x, cap_log2);
+            }
+            if (a.slopes != nullptr) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[j] -= slope * fabsf((float)(p - at - j));
+                for (int j = 0; j < VALUES; ++j) {
+                    x[j] -= slope * fabsf((float)(p - at - j));
+                }
+            }
+            if (!whole) {
+                mask = 0;
+#pragma unroll
+                for (int j = 0; j < VALUES; ++j) {
+                    const bool seen = known && at + j >= lo && at + j < hi;
+                    const bool by_any = RAGGED ? known && at + j >= any_lo && at + j < any_hi : seen;
+                    mask |= (by_any ? 1u : 0u) << j;
+                    x[j] = seen ? x[j] : -INFINITY;
+                }
+            }
+            float most = x[0];
+#pragma unroll
+            for (int j = 1; j < VALUES; ++j) {
+                most = fmaxf(most, x[j]);
+            }
+            if (__any(most > top + 8.0f)) {
+                most = fmaxf(most, __shfl_xor(most, 16));
+                most = fmaxf(most, __shfl_xor(most, 32));
+                most = fmaxf(most, top);
+                keep *= exp2_of(top - most);
+                top = most;
+            }
+            l = sum * keep;
+#pragma unroll
+            for (int j = 0; j < VALUES; ++j) {
+                w[j] = exp2_of(x[j] - top + 6.0f);
+                l += w[j];
+            }
+            if (!M::PARTS || careful || !__any(l != l)) {
+                break;
             }
         }
-        if (!__all((int)base >= lo && (int)base + 32 <= hi && known)) {
-            uint32_t mask = 0;
+        if (__any(keep != 1.0f)) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const bool seen = known && at + j >= lo && at + j < hi;
-                mask |= (seen ? 1u : 0u) << j;
-                x[j] = seen ? x[j] : -INFINITY;
-            }
-            m.clear(v, mask);
-        }
-        float most = x[0];
-#pragma unroll
-        for (int j = 1; j < 8; ++j) {
-            most = fmaxf(most, x[j]);
-        }
-        if (__any(most > top + 8.0f)) {
-            most = fmaxf(most, __shfl_xor(most, 16));
-            most = fmaxf(most, __shfl_xor(most, 32));
-            most = fmaxf(most, top);
-            const float keep = exp2_of(top - most);
-            top = most;
-            l *= keep;
-#pragma unroll
-            for (int i = 0; i < DT; ++i) {
-                o[i] *= keep;
+            for (int j = 0; j < DT; ++j) {
+                o[j] *= keep;
             }
         }
-        float w[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            w[j] = exp2_of(x[j] - top + 6.0f);
-            l += w[j];
+        if (i + 1u < n) {
+            wait_fetches<FETCHES>(); // all but the next tile's keys
+        } else {
+            wait_fetches<0>();
         }
-        m.weigh(o, v, w, c);
+        typename M::V v;
+        m.read_v(v, stage + BYTES, c, g);
+        if (whole) {
+            m.weigh(o, v, w, c);
+        } else {
+            M::clear(v, mask); // (a value that no row sees: 0 x infinity would be NaN)
+            if (RAGGED && __any(!M::finite(v))) {
+                m.weigh_finite(o, v, w, c, lo - at, known ? hi - at : 0);
+            } else {
+                m.weigh(o, v, w, c);
+            }
+        }
+        if (i + 1u < n) {
+            wait_fetches<FETCHES>(); // (the reads of the values)
+            fetch_v(i + 1u, next);
+        }
+        now = next;
+        next = after;
     }
 
     // the waves' results
+    __syncthreads(); // (in the place of their rings)
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
 #pragma unroll
@@ -356,32 +690,35 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_decode_kernel(Decode
     }
     __syncthreads();
     const uint32_t pairs = hd / 2u; // channel pairs of a head
-    const size_t part_floats = (size_t)COLS * (hd + 2u);
-    const size_t slot = (size_t)seq * units + unit;
-    float *mine = args.partials + (slot * args.splits + split) * part_floats;
-    for (uint32_t i = threadIdx.x; i < heads * pairs; i += 256u) {
+    auto write_out = [&](uint32_t of, uint32_t d, float sum, float y0, float y1) {
+        const uint32_t r = first_row + of, query = RAGGED ? r / a.group : 0u;
+        float *out = a.out + (size_t)(row0 + query) * a.out_stride + (size_t)(kvh * a.group + (RAGGED ? r % a.group : r)) * hd + d;
+        out[0] = sum == 0.0f ? 0.0f : y0 / sum;
+        out[1] = sum == 0.0f ? 0.0f : y1 / sum;
+    };
+    auto part_of = [&](uint32_t of) { return args.partials + (slot + of) * part_floats; };
+    for (uint32_t i = threadIdx.x; i < here * pairs; i += THREADS) {
         const uint32_t h = i / pairs, d = 2u * (i % pairs);
         float best = stats[0][0][h];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) {
+        for (int w = 1; w < NW; ++w) {
             best = fmaxf(best, stats[w][0][h]);
         }
         float sum = 0.0f, y0 = 0.0f, y1 = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < NW; ++w) {
             const float f = exp2_of(stats[w][0][h] - best);
             sum += f * stats[w][1][h];
             y0 += f * merged[(w * COLS + h) * PITCH + d];
             y1 += f * merged[(w * COLS + h) * PITCH + d + 1u];
         }
         if (parts == 1u) {
-            float *out = a.out + (size_t)seq * a.out_stride + (size_t)(head0 + h) * hd + d;
-            out[0] = sum == 0.0f ? 0.0f : y0 / sum;
-            out[1] = sum == 0.0f ? 0.0f : y1 / sum;
+            write_out(h, d, sum, y0, y1);
         } else {
-            put2(mine + h * hd + d, y0, y1);
+            float *to = part_of(part);
+            put2(to + h * hd + d, y0, y1);
             if (d == 0u) {
-                put2(mine + COLS * hd + 2u * h, best, sum);
+                put2(to + COLS * hd + 2u * h, best, sum);
             }
         }
     }
@@ -405,49 +742,49 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_decode_kernel(Decode
     if (threadIdx.x == 0u) { // (zero between launches)
         __hip_atomic_store(&args.arrivals[slot], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    const float *first = args.partials + slot * args.splits * part_floats;
-    float *factor = merged; // [head][part], then the sums
-    float *sums = &stats[0][0][0];
-    for (uint32_t h = wave; h < heads; h += 4u) {
-        float best = -3.402823466e38f, sum = 0.0f;
-        for (uint32_t s = lane; s < parts; s += 64u) {
-            float t, n;
-            get2(first + s * part_floats + COLS * hd + 2u * h, t, n);
-            best = fmaxf(best, t);
+    // As many rows at a time as there are threads for, a batch of their parts at a time in LDS:
+    // every load is a trip past the L2, so all of a batch's are on their way at once.
+    const uint32_t at_once = THREADS / pairs;
+    for (uint32_t h0 = 0; h0 < here; h0 += at_once) {
+        const uint32_t some_rows = min(at_once, here - h0), bytes = some_rows * hd * 4u, pieces = (bytes + 1023u) / 1024u;
+        const bool mine = threadIdx.x < some_rows * pairs;
+        const uint32_t row = mine ? threadIdx.x / pairs : 0u, d = 2u * (threadIdx.x % pairs);
+        float best = -3.402823466e38f, sum = 0.0f, y0 = 0.0f, y1 = 0.0f;
+        for (uint32_t s0 = 0; s0 < parts; s0 += PARTS) {
+            const uint32_t some = min((uint32_t)PARTS, parts - s0);
+            __syncthreads(); // (what lay there has been read)
+            for (uint32_t f = wave; f < some * pieces; f += NW) {
+                const uint8_t *from = (const uint8_t *)(part_of(s0 + f / pieces) + h0 * hd);
+                fetch16_past(from + min((f % pieces) * 1024u + lane * 16u, bytes - 16u), lds_address(lds) + f * 1024u);
+            }
+            for (uint32_t i = threadIdx.x; i < some * some_rows; i += THREADS) {
+                float t, of;
+                get2(part_of(s0 + i / some_rows) + COLS * hd + 2u * (h0 + i % some_rows), t, of);
+                joins[i / some_rows][i % some_rows][0] = t;
+                joins[i / some_rows][i % some_rows][1] = of;
+            }
+            wait_fetches<0>();
+            __syncthreads();
+            const float before = best;
+            for (uint32_t k = 0; k < some; ++k) {
+                best = fmaxf(best, joins[k][row][0]);
+            }
+            const float keep = exp2_of(before - best);
+            sum *= keep;
+            y0 *= keep;
+            y1 *= keep;
+#pragma unroll 4
+            for (uint32_t k = 0; k < some; ++k) {
+                const float *of = (const float *)(lds + k * pieces * 1024u) + row * hd + d;
+                const float f = exp2_of(joins[k][row][0] - best);
+                sum += f * joins[k][row][1];
+                y0 += f * of[0];
+                y1 += f * of[1];
+            }
         }
-        for (int x = 32; x > 0; x >>= 1) {
-            best = fmaxf(best, __shfl_xor(best, x));
+        if (mine) {
+            write_out(h0 + row, d, sum, y0, y1);
         }
-        for (uint32_t s = lane; s < parts; s += 64u) {
-            float t, n;
-            get2(first + s * part_floats + COLS * hd + 2u * h, t, n);
-            const float f = exp2_of(t - best);
-            factor[h * DECODE_MAX_SPLITS + s] = f;
-            sum += f * n;
-        }
-        for (int x = 32; x > 0; x >>= 1) {
-            sum += __shfl_xor(sum, x);
-        }
-        if (lane == 0u) {
-            sums[h] = sum;
-        }
-    }
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < heads * pairs; i += 256u) {
-        const uint32_t h = i / pairs, d = 2u * (i % pairs);
-        float y0 = 0.0f, y1 = 0.0f;
-#pragma unroll 8
-        for (uint32_t s = 0; s < parts; ++s) {
-            float u0, u1;
-            get2(first + s * part_floats + h * hd + d, u0, u1);
-            const float f = factor[h * DECODE_MAX_SPLITS + s];
-            y0 += f * u0;
-            y1 += f * u1;
-        }
-        const float sum = sums[h];
-        float *out = a.out + (size_t)seq * a.out_stride + (size_t)(head0 + h) * hd + d;
-        out[0] = sum == 0.0f ? 0.0f : y0 / sum;
-        out[1] = sum == 0.0f ? 0.0f : y1 / sum;
     }
 }
 

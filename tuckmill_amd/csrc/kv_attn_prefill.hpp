@@ -1,4 +1,4 @@
-// Attention of ragged batches of query rows over the paged cache.
+// Attention of ragged batches of many query rows over a paged cache of f16.
 #pragma once
 
 #include "kv_attn_decode.hpp"
@@ -12,58 +12,59 @@ struct PrefillArgs {
     uint32_t splits, tile_bound;
 };
 
-// Sizes of the kernel for pages of T and heads of up to D channels. A row is a query
-// and a head; heads of one key-value head that belong to the same query are
-// neighbours, so a tile of rows reads its keys and values once for all of them.
-template <typename T, int D> struct PrefillShape {
-    static constexpr int E = 16 / (int)sizeof(T);   // elements of a 16-byte unit
-    static constexpr int N = 128 / (int)sizeof(T);  // positions of a step: 64 or 32
-    static constexpr int SUB = N / 32;              // tiles of scores
-    static constexpr int UK = D / E;                // units of a key
-    static constexpr int KS = UK / 2;               // operand pieces of a key
-    static constexpr int DT = D / 32;               // channel tiles
-    static constexpr int BYTES = N * D * (int)sizeof(T); // of a step's keys, and of its values
-    static constexpr int FETCHES = BYTES / 1024 / 4;     // a wave's, of either
+// Sizes of the kernel for heads of up to D channels. A row is a query and a head; heads of one
+// key-value head that belong to the same query are neighbours, so a tile of rows reads its
+// keys and values once for all of them.
+template <int D> struct PrefillShape {
+    static constexpr int E = 8;                  // elements of a 16-byte unit
+    static constexpr int N = 64;                 // positions of a step
+    static constexpr int SUB = N / 32;           // tiles of scores
+    static constexpr int UK = D / E;             // units of a key
+    static constexpr int KS = UK / 2;            // operand pieces of a key
+    static constexpr int DT = D / 32;            // channel tiles
+    static constexpr int BYTES = N * D * 2;      // of a step's keys, and of its values
+    static constexpr int FETCHES = BYTES / 1024 / 4; // a wave's, of either
     static constexpr int SWIZZLE = UK < 16 ? UK - 1 : 15;
 };
 
-// 64 x 16 bytes from the lanes' addresses into 1 KiB of LDS. From inline assembly, and
-// waited for by hand: the compiler's own bookkeeping would order every LDS read
-// behind all such loads in flight.
-__device__ __forceinline__ void fetch16(const void *from, const uint8_t *lds) {
-    const uint32_t m = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)lds);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m), "v"(from) : "memory", "m0");
-}
-
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-// What differs between the two types of page: how a row's q is held, the products
-// and how weights enter the second one.
-template <typename T, int D> struct Rows;
-
-template <int D> struct Rows<_Float16, D> {
-    typedef PrefillShape<_Float16, D> S;
+// How a row's q is held, the products and how weights enter the second one.
+template <int D, bool FULL> struct Rows {
+    typedef PrefillShape<D> S;
     typedef f16x8 Unit;
     Unit hi[S::KS], lo[S::KS]; // q in two parts (22 bits of the row's largest magnitude)
 
     __device__ __forceinline__ float load_q(const float *row, uint32_t h, uint32_t hd, bool live) {
         float top = 0.0f;
-#pragma unroll
-        for (int s = 0; s < S::KS; ++s) {
+        auto read = [&](float (&x)[8], int s) {
+            const uint32_t d = 8u * (2u * s + h);
+            const bool there = live && (FULL || d < hd);
+            const float *from = row + (FULL || d < hd ? d : 0u);
+            const f32x4 y[2] = {*(const f32x4_unaligned *)from, *(const f32x4_unaligned *)(from + 4)};
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const uint32_t d = 8u * (2u * s + h) + j;
-                top = fmaxf(top, live && d < hd ? fabsf(row[d]) : 0.0f);
+                x[j] = there ? y[j / 4][j % 4] : 0.0f;
+            }
+        };
+#pragma unroll
+        for (int s = 0; s < S::KS; ++s) {
+            float x[8];
+            read(x, s);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                top = fmaxf(top, fabsf(x[j]));
             }
         }
         top = fmaxf(top, __shfl_xor(top, 32));
         const int by = scale_bits(top);
 #pragma unroll
         for (int s = 0; s < S::KS; ++s) {
+            float x[8];
+            read(x, s);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const uint32_t d = 8u * (2u * s + h) + j;
-                const float y = live && d < hd ? ldexpf(row[d], by) : 0.0f;
+                const float y = ldexpf(x[j], by);
                 hi[s][j] = (_Float16)y;
                 const float whole = (float)hi[s][j];
                 lo[s][j] = (_Float16)(fabsf(whole) < INFINITY ? y - whole : 0.0f);
@@ -98,49 +99,6 @@ template <int D> struct Rows<_Float16, D> {
     static __device__ __forceinline__ uint32_t v_unit(int i, uint32_t h) { return 2u * i + h; }
 };
 
-template <int D> struct Rows<float, D> {
-    typedef PrefillShape<float, D> S;
-    typedef f32x4 Unit;
-    Unit q[S::KS];
-
-    __device__ __forceinline__ float load_q(const float *row, uint32_t h, uint32_t hd, bool live) {
-#pragma unroll
-        for (int s = 0; s < S::KS; ++s) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t d = 4u * (2u * s + h) + j;
-                q[s][j] = live && d < hd ? row[d] : 0.0f;
-            }
-        }
-        return 1.0f;
-    }
-    __device__ __forceinline__ f32x16 score(f32x16 acc, const Unit &k, int s) const {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(k[j], q[s][j], acc, 0, 0, 0);
-        }
-        return acc;
-    }
-    static constexpr int PIECES = 4; // of the weights: 4 positions for each half
-    struct Weights {
-        float x[16];
-    };
-    static __device__ __forceinline__ void pack(Weights &w, const float (&x)[S::SUB][16]) {
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-            w.x[v] = x[0][v];
-        }
-    }
-    static __device__ __forceinline__ f32x16 weigh(f32x16 acc, const Unit &v, const Weights &w, int i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(v[j], w.x[4 * i + j], acc, 0, 0, 0);
-        }
-        return acc;
-    }
-    static __device__ __forceinline__ uint32_t v_unit(int i, uint32_t h) { return (i / 2) * 4u + 2u * h + (i % 2); }
-};
-
 // A workgroup of four waves per key-value head, tile of 128 rows and share of the
 // positions; each wave has 32 rows and reads the step's keys and values from LDS,
 // where the four fetch them straight from the pages, a step ahead. The products run
@@ -149,14 +107,18 @@ template <int D> struct Rows<float, D> {
 // 16 (a / 2) + 8 h + 4 (a % 2) + b) such that a lane holds of S^T what it hands to O^T = V^T P.
 // In LDS the 16-byte units of a row are swapped by exclusive or with the row's number,
 // which spreads a column of units over the banks.
-template <typename T, int D, bool FULL, int WAVES_PER_SIMD>
+// Bound by the matrix cores where rows are many: a prompt of 8192, 32 heads of 128 channels,
+// 1033 us = 532 TFLOP/s (1064 with both parts of q and of the weights counted); 4001 rows of packed
+// documents of 64 channels with bias and cap 62 us, bound by what happens to each score.
+template <int D, bool FULL, int WAVES_PER_SIMD>
 __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(PrefillArgs args) {
-    typedef PrefillShape<T, D> S;
-    typedef Rows<T, D> R;
+    typedef _Float16 T;
+    typedef PrefillShape<D> S;
+    typedef Rows<D, FULL> R;
     typedef typename R::Unit Unit;
     extern __shared__ __align__(16) uint8_t lds[]; // two stages of keys and values
     __shared__ int range[4][2];
-    __shared__ uint32_t arrived;
+    __shared__ uint32_t arrived, cleaned;
     const AttnArgs &a = args.a;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t c = lane & 31u, h = lane >> 5;
@@ -164,55 +126,11 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
     const uint32_t split = rest % args.splits, index = rest / args.splits;
     const uint32_t hd = FULL ? (uint32_t)D : a.cache.head_dim, shift = a.cache.page_shift;
 
-    // The tile this workgroup has: the sequences' tiles one after the other, the last
-    // (with the most positions to see) first.
-    // (A sequence has rows where its bounds ascend within the batch and no earlier
-    // bound is above its first, so that no two sequences share one.)
-    uint32_t seq = 0, tile = 0, row0 = 0, rows = 0, want = 0xffffffffu;
-    for (int pass = 0; pass < 2; ++pass) {
-        uint32_t before = 0, highest = 0;
-        bool here = false;
-        for (uint32_t s0 = 0; s0 < a.seqs && !here; s0 += 64u) {
-            const uint32_t s = min(s0 + lane, a.seqs - 1u);
-            const uint32_t r0 = a.starts[s], r1 = a.starts[s + 1u];
-            uint32_t above = r0;
-            for (uint32_t x = 1; x < 64u; x <<= 1) {
-                const uint32_t y = __shfl_up(above, x);
-                above = lane >= x ? max(above, y) : above;
-            }
-            above = max(above, highest);
-            highest = __shfl(above, 63);
-            const bool there = s0 + lane < a.seqs && r0 == above && r0 <= r1 && r1 <= a.tokens;
-            const uint32_t n = there ? (r1 - r0) * a.group : 0u, mine = (n + 127u) >> 7;
-            uint32_t upto = mine;
-            for (uint32_t x = 1; x < 64u; x <<= 1) {
-                const uint32_t y = __shfl_up(upto, x);
-                upto += lane >= x ? y : 0u;
-            }
-            if (pass == 1) {
-                const uint64_t found = __ballot(want < before + upto);
-                if (found != 0ull) {
-                    const int at = __builtin_ctzll(found);
-                    seq = s0 + (uint32_t)at;
-                    tile = want - before - (__shfl(upto, at) - __shfl(mine, at));
-                    row0 = __shfl(r0, at);
-                    rows = __shfl(n, at);
-                    here = true;
-                }
-            }
-            before += __shfl(upto, 63);
-        }
-        if (pass == 0) {
-            if (index >= before) {
-                return;
-            }
-            want = before - 1u - index;
-        }
+    uint32_t seq, tile, row0, rows;
+    const uint32_t want = find_tile(a, PREFILL_ROWS, index, seq, tile, row0, rows);
+    if (want == 0xffffffffu) {
+        return;
     }
-    seq = __builtin_amdgcn_readfirstlane(seq);
-    tile = __builtin_amdgcn_readfirstlane(tile);
-    row0 = __builtin_amdgcn_readfirstlane(row0);
-    rows = __builtin_amdgcn_readfirstlane(rows);
 
     // this lane's row
     const int len = seq_len(a, seq), n = (int)(rows / a.group);
@@ -239,6 +157,9 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
     any_hi = __builtin_amdgcn_readfirstlane(any_hi);
     all_lo = __builtin_amdgcn_readfirstlane(all_lo);
     all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+    if (threadIdx.x == 0u) {
+        cleaned = 0u;
+    }
     if (lane == 0u) {
         range[wave][0] = any_lo;
         range[wave][1] = any_hi;
@@ -299,12 +220,12 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
             const uint32_t unit = (lane % S::UK) ^ (at & S::SWIZZLE);
             const uint32_t position = (at & ~12u) | (at & 4u) << 1 | (at & 8u) >> 1;
             const uint32_t d = unit * S::E;
-            fetch16(k + ((base + position) & in_page) * hd + (FULL || d < hd ? d : 0u), k_lds + f * 1024);
+            fetch16(k + ((base + position) & in_page) * hd + (FULL || d < hd ? d : 0u), lds_address(k_lds) + f * 1024);
         }
 #pragma unroll
         for (int f = 0; f < S::FETCHES; ++f) {
             const uint32_t d = (wave * S::FETCHES + f) * 8u + (lane >> 3);
-            fetch16(v + ((FULL ? d : min(d, hd - 1u)) << shift), v_lds + f * 1024);
+            fetch16(v + ((FULL ? d : min(d, hd - 1u)) << shift), lds_address(v_lds) + f * 1024);
         }
     };
 
@@ -317,7 +238,6 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
         }
     }
     float top = -3.402823466e38f, l = 0.0f;
-    bool left_out = false;
     if (s_begin < s_end) {
         look_up(s_begin);
         fetch(s_begin, 0u);
@@ -344,7 +264,7 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
         if (base >= any_hi || base + S::N <= any_lo) {
             continue; // nothing for this wave's rows
         }
-        const uint8_t *k_lds = lds + stage * (2u * S::BYTES), *v_lds = k_lds + S::BYTES;
+        uint8_t *k_lds = lds + stage * (2u * S::BYTES), *v_lds = k_lds + S::BYTES;
         f32x16 acc[S::SUB];
 #pragma unroll
         for (int b = 0; b < S::SUB; ++b) {
@@ -383,21 +303,14 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
         }
         float x[S::SUB][16];
         const int mine = base + 8 * (int)h; // position of value v of tile b: mine + 32 b + 16 (v / 8) + v % 8
-        if (a.softcap > 0.0f) {
 #pragma unroll
-            for (int b = 0; b < S::SUB; ++b) {
+        for (int b = 0; b < S::SUB; ++b) {
 #pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    x[b][v] = cap_log2 * tanh_of(acc[b][v] * to_log2);
-                }
+            for (int v = 0; v < 16; ++v) {
+                x[b][v] = acc[b][v] * to_log2;
             }
-        } else {
-#pragma unroll
-            for (int b = 0; b < S::SUB; ++b) {
-#pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    x[b][v] = acc[b][v] * to_log2;
-                }
+            if (a.softcap > 0.0f) {
+                cap_of(x[b], cap_log2);
             }
         }
         if (a.slopes != nullptr) {
@@ -457,88 +370,88 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
         R::pack(w, x);
         auto v_of = [&](int t, int i) {
             const uint32_t d = 32u * t + c, unit = R::v_unit(i, h);
-            return *(const Unit *)(v_lds + (d * 8u + (unit ^ (d & 7u))) * 16u);
+            return (Unit *)(v_lds + (d * 8u + (unit ^ (d & 7u))) * 16u);
         };
         if (!whole) {
             // A value that is not finite must not reach a row that does not see it through
-            // a weight of zero: such a step's values are added after the loop.
-            float bad = 0.0f;
+            // a weight of zero: it becomes zero in the stage (where the other waves may have
+            // read it before or not), and after the loop the rows that see it are told.
+            Unit bad = {};
 #pragma unroll
             for (int t = 0; t < S::DT; ++t) {
 #pragma unroll
                 for (int i = 0; i < R::PIECES; ++i) {
                     asm volatile("" ::: "memory");
-                    const Unit v = v_of(t, i);
+                    bad = __builtin_elementwise_fma(*v_of(t, i), Unit{}, bad);
+                }
+            }
+            bool any = false;
 #pragma unroll
-                    for (int j = 0; j < S::E; ++j) {
-                        bad += 0.0f * (float)v[j];
+            for (int j = 0; j < S::E; ++j) {
+                any = any || bad[j] != (T)0.0f;
+            }
+            if (__any(any)) {
+                if (lane == 0u) {
+                    cleaned = 1u;
+                }
+#pragma unroll 1
+                for (int t = 0; t < S::DT; ++t) {
+#pragma unroll 1
+                    for (int i = 0; i < R::PIECES; ++i) {
+                        Unit v = *v_of(t, i);
+#pragma unroll
+                        for (int j = 0; j < S::E; ++j) {
+                            v[j] = fabsf((float)v[j]) < INFINITY ? v[j] : (T)0.0f;
+                        }
+                        *v_of(t, i) = v;
                     }
                 }
             }
-            if (__any(bad != 0.0f)) {
-                left_out = true;
-                continue;
-            }
         }
-        Unit v_next = v_of(0, 0);
+        Unit v_next = *v_of(0, 0);
 #pragma unroll
         for (int i = 0; i < R::PIECES * S::DT; ++i) {
             const Unit v = v_next;
             asm volatile("" ::: "memory");
             if (i + 1 < R::PIECES * S::DT) {
-                v_next = v_of((i + 1) % S::DT, (i + 1) / S::DT);
+                v_next = *v_of((i + 1) % S::DT, (i + 1) / S::DT);
             }
             o[i % S::DT] = R::weigh(o[i % S::DT], v, w, i / S::DT);
         }
     }
-    if (left_out) {
-        // The steps in which the wave met a value that is not finite, found again the way the
-        // loop found them, position by position: rare, and as slow as it looks.
-        const float *q_row = a.q + (size_t)row * a.q_stride + (size_t)head * hd;
+    l += __shfl_xor(l, 32);
+    __syncthreads();
+    if (cleaned != 0u) {
+        // Rare, and as slow as it looks: every value that a row of the wave sees.
         for (uint32_t step = s_begin; step < s_end; ++step) {
             const int base = (int)(start + step * S::N);
-            if (base >= any_hi || base + S::N <= any_lo) {
-                continue;
-            }
-            bool known = true, finite = true;
+            bool finite = true;
             for (uint32_t i = lane; i < hd * S::N; i += 64u) {
                 const uint32_t at = (uint32_t)base + i % S::N, page = table[min(at >> shift, last_entry)];
-                known = known && page < a.cache.pages;
                 const T *v = (const T *)a.cache.v + ((size_t)(page < a.cache.pages ? page : 0u) * a.cache.kv_heads + kvh) * page_elements;
                 finite = finite && fabsf((float)v[((i / S::N) << shift) + (at & in_page)]) < INFINITY;
             }
-            if (__all(finite) || (__all(known) && base >= all_lo && base + S::N <= all_hi)) {
+            if (__all(finite)) {
                 continue;
             }
-            for (int i = 0; i < S::N; ++i) {
-                const int at = base + i;
+#pragma unroll 1
+            for (int at = max(base, any_lo); at < min(base + S::N, any_hi); ++at) {
                 const uint32_t page = table[min((uint32_t)at >> shift, last_entry)];
-                if (page >= a.cache.pages) {
-                    continue;
-                }
-                const size_t head_page = ((size_t)page * a.cache.kv_heads + kvh) * page_elements;
-                const T *k = (const T *)a.cache.k + head_page + ((uint32_t)at & in_page) * hd;
-                const T *v = (const T *)a.cache.v + head_page + ((uint32_t)at & in_page);
-                float x = 0.0f;
-                for (uint32_t d = 0; live && d < hd; ++d) {
-                    x = fmaf(q_row[d], (float)k[d], x);
-                }
-                x = a.softcap > 0.0f ? cap_log2 * tanh_of(x * (a.scale / a.softcap)) : x * (a.scale * LOG2E);
-                x -= slope * fabsf((float)(p - at));
-                const bool seen = live && at >= lo && at < hi;
-                const float y = exp2_of(x - top + 6.0f);
+                const bool seen = live && at >= lo && at < hi && page < a.cache.pages;
+                const T *v = (const T *)a.cache.v + ((size_t)(page < a.cache.pages ? page : 0u) * a.cache.kv_heads + kvh) * page_elements +
+                             ((uint32_t)at & in_page);
 #pragma unroll
                 for (int t = 0; t < S::DT; ++t) {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
                         const uint32_t d = 32u * t + 8u * (j / 4) + 4u * h + (j % 4);
-                        o[t][j] += seen && (FULL || d < hd) ? y * (float)v[(FULL ? d : min(d, hd - 1u)) << shift] : 0.0f;
+                        const float x = (float)v[(FULL ? d : min(d, hd - 1u)) << shift];
+                        o[t][j] = seen && !(fabsf(x) < INFINITY) ? NAN : o[t][j];
                     }
                 }
             }
         }
     }
-    l += __shfl_xor(l, 32);
 
     // channel of value v of tile t: 32 t + 8 (v / 4) + 4 h + v % 4
     if (parts == 1u) {

@@ -15,30 +15,53 @@ namespace kv {
 constexpr float LOG2E = 1.4426950408889634f;
 
 typedef q8::f32x4 f32x4;
+typedef f32x4 f32x4_unaligned __attribute__((aligned(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// tanh to a few half steps relative to its value: below 1/2 its series (the first term
-// left out is 5e-9 of it there), above it 1 - 2 t / (1 + t) with t = exp(-2 |y|),
-// which no wave computes whose values are all small (scores well below their cap).
-__device__ __forceinline__ float tanh_of(float y) {
-    const float z = y * y;
-    float s = -0.0014558344f;
-    s = fmaf(s, z, 0.0035921280f);
-    s = fmaf(s, z, -0.0088632355f);
-    s = fmaf(s, z, 0.0218694885f);
-    s = fmaf(s, z, -0.0539682540f);
-    s = fmaf(s, z, 0.1333333333f);
-    s = fmaf(s, z, -0.3333333333f);
-    float r = fmaf(y * z, s, y);
-    const bool large = !(fabsf(y) < 0.5f);
-    if (__any(large)) {
-        const float t = exp2_of(-2.0f * LOG2E * fabsf(y));
-        const float u = (1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t);
-        r = large ? copysignf(u, y) : r;
+// x = cap * tanh(x) for a lane's scores (x = score / cap; cap in units of log2 e), tanh
+// to a few half steps relative to its value: its series below 1/2 (the first term left
+// out is 5e-9 of it there) and below 1/4 (2e-9, five terms); above, (1 - t) / (1 + t) with
+// t = exp(-2 |x|). The ways are chosen for the wave: scores are mostly well below their cap.
+template <int N> __device__ __forceinline__ void cap_of(float (&x)[N], float cap) {
+    float most = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        most = fmaxf(most, fabsf(x[j]));
     }
-    return r;
+    if (__all(most < 0.25f)) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float z = x[j] * x[j];
+            float s = 0.0218694885f;
+            s = fmaf(s, z, -0.0539682540f);
+            s = fmaf(s, z, 0.1333333333f);
+            s = fmaf(s, z, -0.3333333333f);
+            x[j] = cap * fmaf(x[j] * z, s, x[j]);
+        }
+        return;
+    }
+    const bool small = __all(most < 0.5f);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const float z = x[j] * x[j];
+        float s = -0.0014558344f;
+        s = fmaf(s, z, 0.0035921280f);
+        s = fmaf(s, z, -0.0088632355f);
+        s = fmaf(s, z, 0.0218694885f);
+        s = fmaf(s, z, -0.0539682540f);
+        s = fmaf(s, z, 0.1333333333f);
+        s = fmaf(s, z, -0.3333333333f);
+        const float series = fmaf(x[j] * z, s, x[j]);
+        if (!small) {
+            const float t = exp2_of(-2.0f * LOG2E * fabsf(x[j]));
+            const float u = copysignf((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t), x[j]);
+            x[j] = cap * (fabsf(x[j]) < 0.5f ? series : u);
+        } else {
+            x[j] = cap * series;
+        }
+    }
 }
 
 // The power of two that brings a largest magnitude to about 2^13 (none where it is not
@@ -99,6 +122,83 @@ __device__ __forceinline__ void visible(const AttnArgs &a, int len, uint32_t seq
         hi = both > hi ? both : hi;
     }
     hi = hi < len ? hi : len;
+}
+
+// A unit of values in two: what is finite, and 1 where it is not. Where rows of a tile see
+// different positions the first goes into the product with the weights (a weight of
+// zero would not keep an infinity or NaN from a row that does not see it), and the second
+// into a product with 1 for every position that a row sees, which counts the values
+// that make its result NaN.
+template <typename T, typename Unit, int E> __device__ __forceinline__ void part_finite(Unit &v, Unit &wrong) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+        const bool finite = fabsf((float)v[j]) < INFINITY;
+        wrong[j] = (T)(finite ? 0.0f : 1.0f);
+        v[j] = finite ? v[j] : (T)0.0f;
+    }
+}
+
+// Rows of sequence s0 + lane of a ragged batch, for a wave that goes through the sequences 64
+// at a time (`highest`: of the bounds before). A sequence has rows where its bounds ascend
+// within the batch and no earlier bound is above its first, so that no two sequences share
+// one.
+__device__ __forceinline__ uint32_t rows_of(const AttnArgs &a, uint32_t s0, uint32_t &highest) {
+    const uint32_t lane = threadIdx.x & 63u, s = min(s0 + lane, a.seqs - 1u);
+    const uint32_t r0 = a.starts[s], r1 = a.starts[s + 1u];
+    uint32_t above = r0;
+    for (uint32_t x = 1; x < 64u; x <<= 1) {
+        const uint32_t y = __shfl_up(above, x);
+        above = lane >= x ? max(above, y) : above;
+    }
+    above = max(above, highest);
+    highest = __shfl(above, 63);
+    return s0 + lane < a.seqs && r0 == above && r0 <= r1 && r1 <= a.tokens ? r1 - r0 : 0u;
+}
+
+// The index-th tile of the batch's rows (a query and a head of the key-value head's
+// group each), the sequences' tiles one after the other and taken from the last (which
+// has the most positions to see) to the first. Returns the tile's number, or 0xffffffff. Every
+// wave looks for itself, 64 sequences a step.
+__device__ __forceinline__ uint32_t find_tile(const AttnArgs &a, uint32_t tile_rows, uint32_t index, uint32_t &seq,
+                                              uint32_t &tile, uint32_t &row0, uint32_t &rows) {
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t want = 0;
+    seq = tile = row0 = rows = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+        uint32_t before = 0, highest = 0;
+        bool here = false;
+        for (uint32_t s0 = 0; s0 < a.seqs && !here; s0 += 64u) {
+            const uint32_t n = rows_of(a, s0, highest) * a.group, mine = (n + tile_rows - 1u) / tile_rows;
+            uint32_t upto = mine;
+            for (uint32_t x = 1; x < 64u; x <<= 1) {
+                const uint32_t y = __shfl_up(upto, x);
+                upto += lane >= x ? y : 0u;
+            }
+            if (pass == 1) {
+                const uint64_t found = __ballot(want < before + upto);
+                if (found != 0ull) {
+                    const int at = __builtin_ctzll(found);
+                    seq = s0 + (uint32_t)at;
+                    tile = want - before - (__shfl(upto, at) - __shfl(mine, at));
+                    row0 = a.starts[seq];
+                    rows = __shfl(n, at);
+                    here = true;
+                }
+            }
+            before += __shfl(upto, 63);
+        }
+        if (pass == 0) {
+            if (index >= before) {
+                return 0xffffffffu;
+            }
+            want = before - 1u - index;
+        }
+    }
+    seq = __builtin_amdgcn_readfirstlane(seq);
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    row0 = __builtin_amdgcn_readfirstlane(row0);
+    rows = __builtin_amdgcn_readfirstlane(rows);
+    return want;
 }
 
 } // namespace kv

@@ -10,48 +10,79 @@ namespace kv {
 // 16 columns of its matrix operand hold 8 heads in two f16 parts, or 16 in f32.
 inline uint32_t decode_cols(uint32_t type_id) { return type_id == 1u ? 8u : 16u; }
 
-constexpr uint32_t DECODE_MAX_SPLITS = 256;
+// Shares of the positions: one for each CU. (In us, with 256, 512 and 1024 of them: a sequence
+// of 131071 tokens and 8 heads 100, 112, 130; 48 ragged ones up to 8192 156, 158, 155; 16 in
+// f32 with a window of 4096 30, 43, 52: the second workgroup of a CU starts late, and every
+// share is a part to join.)
+constexpr uint32_t DECODE_SHARES = 256;
+constexpr uint64_t DECODE_MAX_GRID = 1u << 23; // (a dimension of a grid is below 2^32 threads)
+constexpr uint32_t DECODE_WAVES = 4; // of a workgroup
+constexpr uint32_t DECODE_MAX_SEQS = 512; // whose work is shared out (every workgroup goes through all of them)
 
 struct AttnPlan {
-    uint32_t splits = 1;     // workgroups that share a sequence's positions
-    uint32_t head_tiles = 1; // workgroups that share a key-value head's query heads
-    uint64_t tile_bound = 0; // tiles of rows, at most
+    bool tiled = false;      // ragged rows: with the prefill kernel (else the decode kernel's)
+    uint32_t shares = 0;     // decode kernel: to make of the positions, 0: one of each unit
+    uint64_t grid = 0;       // workgroups for them, at most
+    uint32_t splits = 1;     // prefill kernel: workgroups that share a tile's positions, at most
+    uint32_t head_tiles = 1; // tiles of a key-value head's query heads
+    uint64_t tile_bound = 0; // prefill kernel: tiles of rows, at most
     uint64_t partial_floats = 0, arrivals = 0; // of the workspace
 };
 
-// One row per sequence. The number of positions is known on the device only: the
-// table's width bounds it, and every workgroup takes an equal share of what there
-// really is (of shares that would be empty the workgroup ends at once).
+// The decode kernel's workgroups: a share each, and what rounding up adds in each unit. How the
+// rows and positions fall to units is known on the device only.
+inline void share_work(AttnPlan &p, uint64_t units, uint32_t cols, uint32_t head_dim, uint64_t positions) {
+    const uint64_t steps = (positions + 63u) / 64u; // (of 64 or 128 positions)
+    const uint64_t most = DECODE_SHARES + units, all = units > most / steps ? most : units * steps;
+    p.shares = DECODE_SHARES;
+    p.grid = all < most ? all : most;
+    // (a unit that is cut has more steps than a share: two workgroups for each full share in it)
+    p.arrivals = 2u * DECODE_SHARES;
+    p.partial_floats = p.arrivals * cols * (head_dim + 2u);
+}
+
+// One row per sequence.
 inline AttnPlan decode_plan(uint32_t type_id, uint32_t seqs, uint32_t q_heads, uint32_t kv_heads,
                             uint32_t head_dim, uint64_t positions) {
     AttnPlan p;
     const uint32_t cols = decode_cols(type_id);
     p.head_tiles = (q_heads / kv_heads + cols - 1u) / cols;
-    const uint64_t units = (uint64_t)seqs * kv_heads * p.head_tiles;
-    uint64_t splits = (2048u + units - 1u) / units;
-    const uint64_t most = (positions + 127u) / 128u; // a step of the four waves each
-    splits = splits < most ? splits : most;
-    p.splits = (uint32_t)(splits < 1u ? 1u : splits > DECODE_MAX_SPLITS ? DECODE_MAX_SPLITS : splits);
-    if (p.splits > 1u) {
-        p.partial_floats = units * p.splits * cols * (head_dim + 2u);
-        p.arrivals = units;
+    if (seqs <= DECODE_MAX_SEQS) {
+        share_work(p, (uint64_t)seqs * kv_heads * p.head_tiles, cols, head_dim, positions);
     }
     return p;
 }
 
 constexpr uint32_t PREFILL_ROWS = 128; // query rows x heads of a workgroup
-constexpr uint32_t PREFILL_MAX_SPLITS = 32;
+constexpr uint32_t PREFILL_MAX_SPLITS = 8;
 constexpr uint64_t PREFILL_MAX_GROUPS = 1u << 23;
+// Up to this many units the decode kernel takes ragged rows. (In us, it and the prefill
+// kernel: at 512 units of 128 channels 25 and 55, at 1024 54 and 67 or 83 and 81, at
+// 2048 135 and 102; of 64 channels at 1024 50 and 60, at 2048 62 and 77; of 256 channels at
+// 2000 137 and 200, at 4000 500 and 357.) Pages of f32 it takes always: their products go at
+// a sixteenth of f16's rate, and its waves of 16 rows fill the card better than tiles of
+// 128 did (1500 rows of 256 channels 94 and 138, 4000 1250 and 1216, 4000 of 64 225 and 264).
+constexpr uint64_t DECODE_MAX_UNITS = 1024;
 
 // Ragged rows. How they fall to sequences is known on the device only: every
 // sequence may have one tile that is not full. Where that leaves few workgroups the
 // positions are shared between several (the parts then go through memory).
-inline AttnPlan prefill_plan(uint32_t seqs, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads,
+inline AttnPlan prefill_plan(uint32_t type_id, uint32_t seqs, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads,
                              uint32_t head_dim, uint64_t positions) {
     AttnPlan p;
     const uint64_t rows = (uint64_t)tokens * (q_heads / kv_heads);
-    const uint64_t per_tile = rows / PREFILL_ROWS + seqs;
-    p.tile_bound = per_tile < rows ? per_tile : rows; // (a tile has a row)
+    auto tiles_of = [&](uint32_t size) { // (a tile has a row)
+        const uint64_t tiles = rows / size + seqs;
+        return tiles < rows ? tiles : rows;
+    };
+    const uint32_t cols = decode_cols(type_id);
+    const uint64_t few = tiles_of(cols) * kv_heads;
+    if (type_id != 1u || few <= DECODE_MAX_UNITS) {
+        share_work(p, few, cols, head_dim, positions);
+        return p;
+    }
+    p.tiled = true;
+    p.tile_bound = tiles_of(PREFILL_ROWS);
     const uint64_t units = p.tile_bound * kv_heads;
     uint64_t splits = units < 256u ? (512u + units - 1u) / units : 1u;
     const uint64_t most = (positions + 255u) / 256u;

@@ -2216,7 +2216,7 @@ int attention(tm_hip_ctx *ctx, const tm_hip_attn *attn, const tm_hip_kv_cache *c
     p.seqs = seqs;
     p.table_stride = table_stride;
     const kv::AttnPlan plan = attn_plan_of(p, ragged ? OP_ATTN_PREFILL : OP_ATTN_DECODE);
-    if (ragged && plan.tile_bound * p.kv_heads * plan.splits > kv::PREFILL_MAX_GROUPS) {
+    if (plan.tile_bound * p.kv_heads * plan.splits > kv::PREFILL_MAX_GROUPS || plan.grid > kv::DECODE_MAX_GRID) {
         return fail(err, cap, TM_HIP_ERR_UNSUPPORTED,
                     "%s: %u rows of %u sequences with %u heads are more than one launch takes", what,
                     tokens, seqs, q_heads);

@@ -39,73 +39,73 @@ kv::AttnArgs attn_args(const Op &op) {
     return a;
 }
 
-template <typename T, int D, int W>
-hipError_t launch_decode_as(hipStream_t stream, hipEvent_t stop, const kv::DecodeArgs &args) {
-    const dim3 grid(args.a.cache.kv_heads * args.head_tiles * args.splits, args.a.seqs);
-    if (args.a.cache.head_dim == (uint32_t)D) {
-        Q8_LAUNCH((kv::attn_decode_kernel<T, D, true, W>), grid, dim3(256), 0, stream, stop, args);
-    } else {
-        Q8_LAUNCH((kv::attn_decode_kernel<T, D, false, W>), grid, dim3(256), 0, stream, stop, args);
-    }
-    return hipGetLastError();
-}
-
-hipError_t launch_decode(hipStream_t stream, hipEvent_t stop, const Op &op) {
-    const KvParams &p = *op.kv;
-    const kv::AttnPlan plan = attn_plan_of(p, op.kind);
-    if (plan.splits > 1u && (p.partials == nullptr || p.arrivals == nullptr)) {
-        return hipErrorInvalidValue;
-    }
-    const kv::DecodeArgs args{attn_args(op), p.partials, p.arrivals, plan.splits, plan.head_tiles};
-    const uint32_t d = p.head_dim;
-    if (p.type_id == 1u) {
-        return d <= 64u    ? launch_decode_as<_Float16, 64, 4>(stream, stop, args)
-               : d <= 128u ? launch_decode_as<_Float16, 128, 3>(stream, stop, args)
-                           : launch_decode_as<_Float16, 256, 2>(stream, stop, args);
-    }
-    return d <= 64u    ? launch_decode_as<float, 64, 3>(stream, stop, args)
-           : d <= 128u ? launch_decode_as<float, 128, 2>(stream, stop, args)
-                       : launch_decode_as<float, 256, 1>(stream, stop, args);
-}
-
-template <typename T, int D, int W>
-hipError_t launch_prefill_as(hipStream_t stream, hipEvent_t stop, const kv::PrefillArgs &args) {
-    constexpr int LDS = 4 * kv::PrefillShape<T, D>::BYTES;
-    static_assert(LDS >= 128 * (int)(kv::PREFILL_MAX_SPLITS + 1u) * 4, "factors and sums of a join");
-    const dim3 grid(args.a.cache.kv_heads * args.splits * args.tile_bound);
-    const bool full = args.a.cache.head_dim == (uint32_t)D;
-    const void *kernel = full ? (const void *)kv::attn_prefill_kernel<T, D, true, W>
-                              : (const void *)kv::attn_prefill_kernel<T, D, false, W>;
-    if (LDS >= 65536) { // (with a few static words) beyond what a launch may ask for without saying so
-        const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-        if (e != hipSuccess) {
-            return e;
+// A launch with LDS bytes of dynamic LDS: beyond 64 KiB (the few static words counted in)
+// a kernel has to be told once that it may.
+template <uint32_t LDS, auto KERNEL, typename Args>
+hipError_t launch_lds(hipStream_t stream, hipEvent_t stop, dim3 grid, dim3 block, const Args &args) {
+    if (LDS + 1024u > 65536u) {
+        static const hipError_t told =
+            hipFuncSetAttribute((const void *)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, (int)LDS);
+        if (told != hipSuccess) {
+            return told;
         }
     }
-    if (full) {
-        Q8_LAUNCH((kv::attn_prefill_kernel<T, D, true, W>), grid, dim3(256), LDS, stream, stop, args);
-    } else {
-        Q8_LAUNCH((kv::attn_prefill_kernel<T, D, false, W>), grid, dim3(256), LDS, stream, stop, args);
-    }
+    Q8_LAUNCH(KERNEL, grid, block, LDS, stream, stop, args);
     return hipGetLastError();
+}
+
+template <typename T, int D, bool RAGGED>
+hipError_t launch_decode_as(hipStream_t stream, hipEvent_t stop, const kv::DecodeArgs &args, uint64_t grid_x) {
+    const dim3 grid = args.shares != 0u ? dim3((uint32_t)grid_x) : dim3(args.a.cache.kv_heads * args.head_tiles, args.a.seqs);
+    constexpr uint32_t LDS = kv::DECODE_WAVES * 2u * 64u * D; // a tile's keys are 64 D bytes in either type
+    const dim3 block(64u * kv::DECODE_WAVES);
+    return args.a.cache.head_dim == (uint32_t)D
+               ? launch_lds<LDS, kv::attn_decode_kernel<T, D, true, RAGGED>>(stream, stop, grid, block, args)
+               : launch_lds<LDS, kv::attn_decode_kernel<T, D, false, RAGGED>>(stream, stop, grid, block, args);
+}
+
+// A row per sequence, or (RAGGED) sequences of few rows.
+template <bool RAGGED> hipError_t launch_decode(hipStream_t stream, hipEvent_t stop, const Op &op) {
+    const KvParams &p = *op.kv;
+    const kv::AttnPlan plan = attn_plan_of(p, op.kind);
+    if (plan.shares != 0u && (p.partials == nullptr || p.arrivals == nullptr || plan.grid > kv::DECODE_MAX_GRID)) {
+        return hipErrorInvalidValue;
+    }
+    const kv::DecodeArgs args{attn_args(op), p.partials, p.arrivals, plan.shares, plan.head_tiles};
+    const uint32_t d = p.head_dim;
+    if (p.type_id == 1u) {
+        return d <= 64u    ? launch_decode_as<_Float16, 64, RAGGED>(stream, stop, args, plan.grid)
+               : d <= 128u ? launch_decode_as<_Float16, 128, RAGGED>(stream, stop, args, plan.grid)
+                           : launch_decode_as<_Float16, 256, RAGGED>(stream, stop, args, plan.grid);
+    }
+    return d <= 64u    ? launch_decode_as<float, 64, RAGGED>(stream, stop, args, plan.grid)
+           : d <= 128u ? launch_decode_as<float, 128, RAGGED>(stream, stop, args, plan.grid)
+                       : launch_decode_as<float, 256, RAGGED>(stream, stop, args, plan.grid);
+}
+
+template <int D, int W> hipError_t launch_prefill_as(hipStream_t stream, hipEvent_t stop, const kv::PrefillArgs &args) {
+    constexpr uint32_t LDS = 4u * kv::PrefillShape<D>::BYTES;
+    static_assert(LDS >= 128u * (kv::PREFILL_MAX_SPLITS + 1u) * 4u, "factors and sums of a join");
+    const dim3 grid(args.a.cache.kv_heads * args.splits * args.tile_bound);
+    return args.a.cache.head_dim == (uint32_t)D
+               ? launch_lds<LDS, kv::attn_prefill_kernel<D, true, W>>(stream, stop, grid, dim3(256), args)
+               : launch_lds<LDS, kv::attn_prefill_kernel<D, false, W>>(stream, stop, grid, dim3(256), args);
 }
 
 hipError_t launch_prefill(hipStream_t stream, hipEvent_t stop, const Op &op) {
     const KvParams &p = *op.kv;
     const kv::AttnPlan plan = attn_plan_of(p, op.kind);
+    if (!plan.tiled) {
+        return launch_decode<true>(stream, stop, op);
+    }
     if (plan.splits > 1u && (p.partials == nullptr || p.arrivals == nullptr)) {
         return hipErrorInvalidValue;
     }
     const kv::PrefillArgs args{attn_args(op), p.partials, p.arrivals, plan.splits, (uint32_t)plan.tile_bound};
     const uint32_t d = p.head_dim;
-    if (p.type_id == 1u) {
-        return d <= 64u    ? launch_prefill_as<_Float16, 64, 2>(stream, stop, args)
-               : d <= 128u ? launch_prefill_as<_Float16, 128, 2>(stream, stop, args)
-                           : launch_prefill_as<_Float16, 256, 1>(stream, stop, args);
-    }
-    return d <= 64u    ? launch_prefill_as<float, 64, 2>(stream, stop, args)
-           : d <= 128u ? launch_prefill_as<float, 128, 2>(stream, stop, args)
-                       : launch_prefill_as<float, 256, 1>(stream, stop, args);
+    return d <= 64u    ? launch_prefill_as<64, 2>(stream, stop, args)
+           : d <= 128u ? launch_prefill_as<128, 2>(stream, stop, args)
+                       : launch_prefill_as<256, 1>(stream, stop, args);
 }
 
 hipError_t launch_rope(hipStream_t stream, hipEvent_t stop, const Op &op) {
@@ -187,7 +187,7 @@ hipError_t tmdev::launch_kv(hipStream_t stream, hipEvent_t stop, const Op &op) {
     case OP_ROPE_STORE:
         return launch_rope(stream, stop, op);
     case OP_ATTN_DECODE:
-        return launch_decode(stream, stop, op);
+        return launch_decode<false>(stream, stop, op);
     case OP_ATTN_PREFILL:
         return launch_prefill(stream, stop, op);
     case OP_LOGITS:

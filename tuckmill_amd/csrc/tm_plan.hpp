@@ -103,7 +103,7 @@ inline kv::AttnPlan attn_plan_of(const KvParams &p, OpKind kind) {
         return kv::decode_plan(p.type_id, p.seqs, p.q_heads, p.kv_heads, p.head_dim,
                                (uint64_t)p.table_stride << p.page_shift);
     }
-    return kv::prefill_plan(p.seqs, p.tokens, p.q_heads, p.kv_heads, p.head_dim,
+    return kv::prefill_plan(p.type_id, p.seqs, p.tokens, p.q_heads, p.kv_heads, p.head_dim,
                             (uint64_t)p.table_stride << p.page_shift);
 }
 
