@@ -32,10 +32,10 @@ template <int D, bool FULL> struct Tile<_Float16, D, FULL> {
     static constexpr int DT = D / 16;     // channel tiles
     static constexpr int HALVES = 2;      // of 16 keys each in a tile's stage
     static constexpr bool PARTS = true;
-    typedef f16x8 K[2][KS];
-    typedef f16x8 V[DT];
+    typedef f16x8 Unit;
+    typedef Unit K[2]; // of a piece
     typedef f32x4 S[2];
-    f16x8 q[KS];
+    Unit q[KS];
 
     // The row's q, scaled by a power of two to a largest magnitude of about 2^13, as
     // f16 parts (22 bits of that magnitude); returns the inverse scale. What is
@@ -73,38 +73,19 @@ template <int D, bool FULL> struct Tile<_Float16, D, FULL> {
     static constexpr __device__ __forceinline__ uint32_t k_position(uint32_t at) {
         return 8u * ((at & 15u) >> 2) + (at & 3u) + 4u * (at >> 4);
     }
-    __device__ __forceinline__ void read_k(K &k, const uint8_t *stage, uint32_t c, uint32_t g, uint32_t hd) const {
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const uint32_t unit = 4u * s + g;
-            const bool in = FULL || 8u * unit < hd;
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const uint32_t at = 16u * t + c;
-                const f16x8 x = *(const f16x8 *)(stage + (at * UK + (unit ^ (at & SWIZZLE))) * 16u);
-                k[t][s] = in ? x : f16x8{};
-            }
-        }
-    }
-    // channel 16 t + c, positions 8 g + 0..7
-    __device__ __forceinline__ void read_v(V &v, const uint8_t *stage, uint32_t c, uint32_t g) const {
-#pragma unroll
-        for (int t = 0; t < DT; ++t) {
-            const uint32_t d = 16u * t + c;
-            v[t] = *(const f16x8 *)(stage + (d * 4u + (g ^ ((d >> 2) & 3u))) * 16u);
-        }
-    }
-    __device__ __forceinline__ void products(S &acc, const K &k) const {
+    static __device__ __forceinline__ void read_k(K &k, const uint8_t *stage, uint32_t c, uint32_t g, uint32_t hd, int s) {
+        const uint32_t unit = 4u * s + g;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            const uint32_t at = 16u * t + c;
+            const Unit x = *(const Unit *)(stage + (at * UK + (unit ^ (at & SWIZZLE))) * 16u);
+            k[t] = FULL || 8u * unit < hd ? x : Unit{};
         }
+    }
+    __device__ __forceinline__ void product(S &acc, const K &k, int s) const {
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][s], q[s], acc[t], 0, 0, 0);
-            }
+        for (int t = 0; t < 2; ++t) {
+            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t], q[s], acc[t], 0, 0, 0);
         }
     }
     // Both parts of the row: columns c and c + 8 of 16. Where a key is infinite the first
@@ -118,65 +99,18 @@ template <int D, bool FULL> struct Tile<_Float16, D, FULL> {
         }
     }
     // the part of the weights that the column stands for
-    static __device__ __forceinline__ f16x8 part_of(const float (&w)[VALUES], uint32_t c) {
+    typedef Unit Weights;
+    static __device__ __forceinline__ Weights pack(const float (&w)[VALUES], uint32_t c) {
         const float second = c < 8u ? 0.0f : -1.0f;
-        f16x8 p;
+        Weights p;
 #pragma unroll
         for (int j = 0; j < VALUES; ++j) {
             p[j] = (_Float16)fmaf((float)(_Float16)w[j], second, w[j]);
         }
         return p;
     }
-    __device__ __forceinline__ void weigh(f32x4 (&o)[DT], const V &v, const float (&w)[VALUES], uint32_t c) const {
-        const f16x8 p = part_of(w, c);
-#pragma unroll
-        for (int t = 0; t < DT; ++t) {
-            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], p, o[t], 0, 0, 0);
-        }
-    }
-    // weigh() where values that are not finite meet rows that do not see them (part_finite):
-    // a row sees the lane's positions from <= j < upto.
-    __device__ __forceinline__ void weigh_finite(f32x4 (&o)[DT], const V &v, const float (&w)[VALUES], uint32_t c, int from,
-                                                 int upto) const {
-        const f16x8 p = part_of(w, c);
-        f16x8 ones;
-#pragma unroll
-        for (int j = 0; j < VALUES; ++j) {
-            ones[j] = (_Float16)(j >= from && j < upto ? 1.0f : 0.0f);
-        }
-#pragma unroll
-        for (int t = 0; t < DT; ++t) {
-            f16x8 clean = v[t], wrong;
-            part_finite<_Float16, f16x8, 8>(clean, wrong);
-            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(clean, p, o[t], 0, 0, 0);
-            f32x4 count = {0.0f, 0.0f, 0.0f, 0.0f};
-            count = __builtin_amdgcn_mfma_f32_16x16x32_f16(wrong, ones, count, 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                o[t][i] = count[i] > 0.0f ? NAN : o[t][i];
-            }
-        }
-    }
-    // positions whose bit of `mask` is not set as zeros (0 x infinity would be NaN)
-    static __device__ __forceinline__ void clear(V &v, uint32_t mask) {
-#pragma unroll
-        for (int t = 0; t < DT; ++t) {
-#pragma unroll
-            for (int j = 0; j < VALUES; ++j) {
-                v[t][j] = (mask >> j) & 1u ? v[t][j] : (_Float16)0.0f;
-            }
-        }
-    }
-    static __device__ __forceinline__ bool finite(const V &v) {
-        float bad = 0.0f;
-#pragma unroll
-        for (int t = 0; t < DT; ++t) {
-#pragma unroll
-            for (int j = 0; j < VALUES; ++j) {
-                bad += 0.0f * (float)v[t][j];
-            }
-        }
-        return bad == 0.0f;
+    static __device__ __forceinline__ f32x4 weigh(f32x4 o, const Unit &v, const Weights &w) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w, o, 0, 0, 0);
     }
     static __device__ __forceinline__ float whole(float x) { return x + ror8(x); }
 };
@@ -189,10 +123,10 @@ template <int D, bool FULL> struct Tile<float, D, FULL> {
     static constexpr int DT = D / 16;
     static constexpr int HALVES = 1;
     static constexpr bool PARTS = false;
-    typedef f32x4 K[KS];
-    typedef f32x4 V[DT];
-    typedef f32x4 S;
-    f32x4 q[KS];
+    typedef f32x4 Unit;
+    typedef Unit K;
+    typedef f32x4 S[2]; // two sums: a product waits for the one before it in its sum
+    Unit q[KS];
 
     __device__ __forceinline__ float load_q(const float *row, uint32_t, uint32_t g, uint32_t hd, bool live, float sign) {
 #pragma unroll
@@ -204,85 +138,31 @@ template <int D, bool FULL> struct Tile<float, D, FULL> {
         return 1.0f;
     }
     static constexpr __device__ __forceinline__ uint32_t k_position(uint32_t at) { return at; }
-    __device__ __forceinline__ void read_k(K &k, const uint8_t *stage, uint32_t c, uint32_t g, uint32_t hd) const {
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const uint32_t unit = 4u * s + g;
-            const f32x4 x = *(const f32x4 *)(stage + (c * UK + (unit ^ (c & SWIZZLE))) * 16u);
-            k[s] = FULL || 4u * unit < hd ? x : f32x4{};
-        }
+    static __device__ __forceinline__ void read_k(K &k, const uint8_t *stage, uint32_t c, uint32_t g, uint32_t hd, int s) {
+        const uint32_t unit = 4u * s + g;
+        const Unit x = *(const Unit *)(stage + (c * UK + (unit ^ (c & SWIZZLE))) * 16u);
+        k = FULL || 4u * unit < hd ? x : Unit{};
     }
-    __device__ __forceinline__ void read_v(V &v, const uint8_t *stage, uint32_t c, uint32_t g) const {
+    __device__ __forceinline__ void product(S &acc, const K &k, int s) const {
 #pragma unroll
-        for (int t = 0; t < DT; ++t) {
-            const uint32_t d = 16u * t + c;
-            v[t] = *(const f32x4 *)(stage + (d * 4u + (g ^ ((d >> 2) & 3u))) * 16u);
+        for (int j = 0; j < 4; ++j) {
+            acc[j % 2] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[j], q[s][j], acc[j % 2], 0, 0, 0);
         }
-    }
-    __device__ __forceinline__ void products(S &acc, const K &k) const {
-        // (two sums: a product waits for the one before it in its sum)
-        f32x4 even = {0.0f, 0.0f, 0.0f, 0.0f}, odd = even;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-#pragma unroll
-            for (int j = 0; j < 4; j += 2) {
-                even = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][j], q[s][j], even, 0, 0, 0);
-                odd = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][j + 1], q[s][j + 1], odd, 0, 0, 0);
-            }
-        }
-        acc = even + odd;
     }
     static __device__ __forceinline__ void scores(float (&x)[VALUES], const S &acc, uint32_t, bool) {
 #pragma unroll
         for (int j = 0; j < VALUES; ++j) {
-            x[j] = acc[j];
+            x[j] = acc[0][j] + acc[1][j];
         }
     }
-    __device__ __forceinline__ void weigh(f32x4 (&o)[DT], const V &v, const float (&w)[VALUES], uint32_t) const {
+    typedef Unit Weights;
+    static __device__ __forceinline__ Weights pack(const float (&w)[VALUES], uint32_t) { return Unit{w[0], w[1], w[2], w[3]}; }
+    static __device__ __forceinline__ f32x4 weigh(f32x4 o, const Unit &v, const Weights &w) {
 #pragma unroll
-        for (int j = 0; j < VALUES; ++j) {
-#pragma unroll
-            for (int t = 0; t < DT; ++t) {
-                o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[t][j], w[j], o[t], 0, 0, 0);
-            }
+        for (int j = 0; j < 4; ++j) {
+            o = __builtin_amdgcn_mfma_f32_16x16x4f32(v[j], w[j], o, 0, 0, 0);
         }
-    }
-    __device__ __forceinline__ void weigh_finite(f32x4 (&o)[DT], const V &v, const float (&w)[VALUES], uint32_t, int from,
-                                                 int upto) const {
-#pragma unroll
-        for (int t = 0; t < DT; ++t) {
-            f32x4 clean = v[t], wrong, count = {0.0f, 0.0f, 0.0f, 0.0f};
-            part_finite<float, f32x4, 4>(clean, wrong);
-#pragma unroll
-            for (int j = 0; j < VALUES; ++j) {
-                o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(clean[j], w[j], o[t], 0, 0, 0);
-                count = __builtin_amdgcn_mfma_f32_16x16x4f32(wrong[j], j >= from && j < upto ? 1.0f : 0.0f, count, 0, 0, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                o[t][i] = count[i] > 0.0f ? NAN : o[t][i];
-            }
-        }
-    }
-    static __device__ __forceinline__ void clear(V &v, uint32_t mask) {
-#pragma unroll
-        for (int t = 0; t < DT; ++t) {
-#pragma unroll
-            for (int j = 0; j < VALUES; ++j) {
-                v[t][j] = (mask >> j) & 1u ? v[t][j] : 0.0f;
-            }
-        }
-    }
-    static __device__ __forceinline__ bool finite(const V &v) {
-        float bad = 0.0f;
-#pragma unroll
-        for (int t = 0; t < DT; ++t) {
-#pragma unroll
-            for (int j = 0; j < VALUES; ++j) {
-                bad += 0.0f * v[t][j];
-            }
-        }
-        return bad == 0.0f;
+        return o;
     }
     static __device__ __forceinline__ float whole(float x) { return x; }
 };
@@ -331,6 +211,18 @@ template <int N> __device__ __forceinline__ void wait_fetches() {
     asm volatile("" ::: "memory");
 }
 
+// Stages of a wave in LDS: two, where one query per sequence waits for memory (48 ragged sequences
+// of 128 channels 155 us, with one 162), or one for keys and values in turn, which leaves room for
+// more workgroups, where several rows share them (2000 f32 rows of 128 channels 115 us, with two
+// 139) or a stage is large (1500 of 256 channels 69, with two 95).
+template <typename T, int D, bool RAGGED> struct DecodeShape {
+    static constexpr int RING = RAGGED || D > 128 ? 1 : 2;
+    static constexpr int COLS = sizeof(T) == 2 ? 8 : 16, PITCH = D + 4;
+    static constexpr int BYTES = 64 * D;          // keys or values of a tile
+    static constexpr int RESULTS = COLS * PITCH * 4;
+    static constexpr int LDS = DECODE_WAVES * (RING * BYTES > RESULTS ? RING * BYTES : RESULTS);
+};
+
 // A unit of work is a key-value head and a tile of rows; a row is a query and a head of
 // the key-value head's group (RAGGED: the rows of tm_hip_attn_prefill where a sequence
 // has few, else one query a sequence). The positions of all units, in steps of a tile for
@@ -338,9 +230,9 @@ template <int N> __device__ __forceinline__ void wait_fetches() {
 // busy: sequences of any lengths end together. A share lies in one unit (one that ran
 // on into the next unit would save 1% of the steps and cost a second prologue and join).
 // The keys and values of a tile of positions come straight from the pages into the wave's
-// own LDS; each half (keys, then values) is fetched again as soon as it has been
-// read, so that one of the two is always on its way, the waves never wait for
-// each other before the end, and registers do not bound what is in flight. A fetch
+// own LDS; a stage is fetched again as soon as it has been read, so that keys or values
+// are always on their way, the waves never wait for each other before the end, and
+// registers do not bound what is in flight. A fetch
 // costs no vector instruction: the lanes' offsets stay the same from tile to
 // tile, pages and places move the scalar base.
 // The softmax runs over one pass: weights are 2^(x - m + 6) with a reference m
@@ -353,16 +245,22 @@ template <int N> __device__ __forceinline__ void wait_fetches() {
 // channels in f16, 100 us = 5.4 TB/s; 777 tokens 9 us, of which the launch is most. Short calls
 // are bound by the way through the code, every line of which is fetched once: loads of q in
 // wide pieces and a rolled join (20 KB of code for 30) took 16 sequences in f32 from 57 to 30 us.
+// Bound by the f32 matrix cores where f32 rows are many: two sequences of 2000 rows, 16 heads of 128
+// channels, 347 us.
 template <typename T, int D, bool FULL, bool RAGGED>
-__global__ __launch_bounds__(64 * DECODE_WAVES, D <= 128 ? 2 : 1) void attn_decode_kernel(DecodeArgs args) {
+__global__ __launch_bounds__(64 * DECODE_WAVES, 2) void attn_decode_kernel(DecodeArgs args) {
     typedef Tile<T, D, FULL> M;
-    constexpr int COLS = M::COLS, DT = M::DT, PITCH = D + 4, VALUES = M::VALUES, TOKENS = 4 * VALUES;
-    constexpr int NW = DECODE_WAVES, THREADS = 64 * NW;
-    constexpr int BYTES = TOKENS * D * (int)sizeof(T), FETCHES = BYTES / 1024; // keys or values of a tile
+    typedef DecodeShape<T, D, RAGGED> Shape;
+    typedef typename M::Unit Unit;
+    constexpr int COLS = M::COLS, DT = M::DT, KS = M::KS, PITCH = Shape::PITCH, VALUES = M::VALUES, TOKENS = 4 * VALUES;
+    constexpr int NW = DECODE_WAVES, RING = Shape::RING, THREADS = 64 * NW;
+    constexpr int PIECES = RING == 2 ? 64 : 4; // of keys and values on their way from LDS at a time
+    constexpr int BYTES = Shape::BYTES, FETCHES = BYTES / 1024; // keys or values of a tile
     constexpr int PAGES = TOKENS / 16, KINDS = FETCHES / M::HALVES; // of lane offsets of keys
-    constexpr int PARTS = D <= 64 ? 16 : 32; // that a join takes at a time, of 2 KiB at most
+    // that a join takes at a time, of 8 bytes for each thread
+    constexpr int PARTS = Shape::LDS / (8 * THREADS) < 32 ? Shape::LDS / (8 * THREADS) : 32;
     extern __shared__ __align__(16) uint8_t lds[]; // keys and values of each wave; at the end the waves' results
-    static_assert(COLS * PITCH * 4 <= 2 * BYTES && PARTS * 2048 <= NW * 2 * BYTES && 8 * THREADS <= 2048, "results");
+    static_assert(TOKENS * D * (int)sizeof(T) == BYTES && COLS == Shape::COLS, "results");
     float *merged = (float *)lds;
     __shared__ float stats[NW][2][COLS];
     __shared__ float joins[PARTS][COLS][2];
@@ -374,8 +272,8 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, D <= 128 ? 2 : 1) void attn_deco
     const size_t part_floats = (size_t)COLS * (hd + 2u);
     const uint32_t last_entry = a.table_stride - 1u, in_page = (1u << shift) - 1u;
     const uint32_t page_elements = hd << shift;
-    const uint8_t *stage = lds + wave * (2u * BYTES);
-    const uint32_t k_lds = lds_address(stage), v_lds = k_lds + BYTES;
+    uint8_t *stage = lds + wave * (RING * BYTES), *v_stage = stage + (RING - 1) * BYTES;
+    const uint32_t k_lds = lds_address(stage), v_lds = lds_address(v_stage);
     // A fetch of keys is rows 64 / UK of the stage, all within 16 positions of the tile.
     constexpr uint32_t ROWS = 64u / M::UK;
     uint32_t k_offset[KINDS];
@@ -388,7 +286,7 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, D <= 128 ? 2 : 1) void attn_deco
     const uint32_t v_row = lane >> 2, v_position = ((lane & 3u) ^ ((v_row >> 2) & 3u)) * M::E;
 
     // What there is to do, and this workgroup's share of it.
-    auto units_of = [&](uint32_t s, uint32_t n) { // of a sequence of n rows
+    auto units_of = [&](uint32_t n) { // of a sequence of n rows
         return RAGGED ? (n * a.group + COLS - 1u) / COLS * a.cache.kv_heads : a.cache.kv_heads * args.head_tiles;
     };
     // Steps of a unit: of the positions that the sequence's query sees, or (RAGGED, where
@@ -410,19 +308,24 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, D <= 128 ? 2 : 1) void attn_deco
         // 64 sequences, one a lane: its rows, a unit's steps, and the sum up to its end: of steps, or
         // (once the size of a share is known) of shares, and in the high half of those that
         // are not all of their unit
-        uint32_t s0 = 0, highest = 0, rows_up_to = 0, rows_here = 0, steps_here = 0, size = 0;
+        uint32_t s0 = 0, highest = 0, rows_up_to = 0, first_here = 0, rows_here = 0, steps_here = 0, size = 0;
         uint64_t before = 0, upto = 0; // `before`: of the sequences before s0
-        auto look = [&]() {
-            rows_up_to = highest;
-            const uint32_t s = min(s0 + lane, a.seqs - 1u);
-            rows_here = RAGGED ? rows_of(a, s0, rows_up_to) : s0 + lane < a.seqs ? 1u : 0u;
-            steps_here = rows_here != 0u ? steps_of(s, rows_here) : 0u;
+        auto add_up = [&]() {
             const uint64_t shares = size != 0u ? (steps_here + size - 1u) / size : 0u;
-            upto = (uint64_t)units_of(s, rows_here) * (size == 0u ? steps_here : shares > 1u ? shares | shares << 32 : shares);
+            upto = (uint64_t)units_of(rows_here) * (size == 0u ? steps_here : shares > 1u ? shares | shares << 32 : shares);
             for (uint32_t x = 1; x < 64u; x <<= 1) {
                 const uint64_t y = __shfl_up(upto, x);
                 upto += lane >= x ? y : 0u;
             }
+        };
+        auto look = [&]() {
+            rows_up_to = highest;
+            const uint32_t s = min(s0 + lane, a.seqs - 1u);
+            first_here = s;
+            rows_here = RAGGED ? rows_of(a, s0, rows_up_to, first_here) : s0 + lane < a.seqs ? 1u : 0u;
+            steps_here = steps_of(s, rows_here);
+            steps_here = rows_here != 0u ? steps_here : 0u;
+            add_up();
         };
         auto look_on = [&]() {
             before += __shfl(upto, 63);
@@ -436,9 +339,13 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, D <= 128 ? 2 : 1) void attn_deco
         }
         size = (uint32_t)((before + __shfl(upto, 63) + args.shares - 1u) / args.shares);
         size = __builtin_amdgcn_readfirstlane(max(size, 1u));
-        s0 = highest = 0;
         before = 0;
-        look();
+        if (s0 == 0u) {
+            add_up();
+        } else {
+            s0 = highest = 0;
+            look();
+        }
         uint64_t found;
         while ((found = __ballot(blockIdx.x < (uint32_t)(before + upto))) == 0ull) {
             if (s0 + 64u >= a.seqs) {
@@ -450,7 +357,7 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, D <= 128 ? 2 : 1) void attn_deco
         seq = s0 + (uint32_t)at;
         parts = (__shfl(steps_here, at) + size - 1u) / size;
         rows = __shfl(rows_here, at) * a.group;
-        row0 = RAGGED ? a.starts[seq] : seq;
+        row0 = __shfl(first_here, at);
         before += at > 0 ? __shfl(upto, at - 1) : 0u;
         const uint32_t index = blockIdx.x - (uint32_t)before, unit = index / parts;
         part = index % parts;
@@ -549,7 +456,9 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, D <= 128 ? 2 : 1) void attn_deco
     if (n > 0u) {
         now = look_up(0u);
         fetch_k(0u, now);
-        fetch_v(0u, now);
+        if constexpr (RING == 2) {
+            fetch_v(0u, now);
+        }
         next = look_up(1u);
     }
 
@@ -567,25 +476,51 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, D <= 128 ? 2 : 1) void attn_deco
         o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     float top = -3.402823466e38f, l = 0.0f;
+    bool cleaned = false;
 
     for (uint32_t i = 0; i < n; ++i) {
         const uint32_t base = start + TOKENS * (t0 + i);
         const Pages after = look_up(i + 2u);
-        typename M::S acc;
+        typename M::S acc = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+        wait_fetches<(RING - 1) * FETCHES>(); // all but this tile's values
         {
-            wait_fetches<FETCHES>(); // all but this tile's values
-            typename M::K k;
-            m.read_k(k, stage, c, g, hd);
-            m.products(acc, k);
+            // (where registers are short: a few pieces are read while those before them are
+            // multiplied, and no earlier)
+            constexpr int AT_ONCE = PIECES < KS ? PIECES : KS;
+            typename M::K k[AT_ONCE], ahead[AT_ONCE];
+#pragma unroll
+            for (int s = 0; s < AT_ONCE; ++s) {
+                M::read_k(ahead[s], stage, c, g, hd, s);
+            }
+#pragma unroll
+            for (int s0 = 0; s0 < KS; s0 += AT_ONCE) {
+#pragma unroll
+                for (int s = 0; s < AT_ONCE; ++s) {
+                    __builtin_memcpy(&k[s], &ahead[s], sizeof(k[s]));
+                }
+                if (s0 + AT_ONCE < KS) {
+                    asm volatile("" ::: "memory");
+#pragma unroll
+                    for (int s = 0; s < AT_ONCE; ++s) {
+                        M::read_k(ahead[s], stage, c, g, hd, s0 + AT_ONCE + s);
+                    }
+                } else if constexpr (RING == 1) {
+                    wait_fetches<0>(); // (the reads of the keys)
+                    fetch_v(i, now);
+                }
+#pragma unroll
+                for (int s = 0; s < AT_ONCE; ++s) {
+                    m.product(acc, k[s], s0 + s);
+                }
+            }
         }
-        if (i + 1u < n) {
+        if (RING == 2 && i + 1u < n) {
             wait_fetches<FETCHES>(); // (the reads of the keys)
             fetch_k(i + 1u, next);
         }
         const bool known = (PAGES == 1 || g < 2u ? now.id[0] : now.id[PAGES - 1]) < a.cache.pages;
         const int at = (int)(base + VALUES * g);
         const bool whole = __all((int)base >= all_lo && (int)base + TOKENS <= all_hi && known);
-        uint32_t mask = 0;
         float w[VALUES];
         float keep = 1.0f, sum = l;
         for (bool careful = false;; careful = true) {
@@ -607,13 +542,9 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, D <= 128 ? 2 : 1) void attn_deco
                 }
             }
             if (!whole) {
-                mask = 0;
 #pragma unroll
                 for (int j = 0; j < VALUES; ++j) {
-                    const bool seen = known && at + j >= lo && at + j < hi;
-                    const bool by_any = RAGGED ? known && at + j >= any_lo && at + j < any_hi : seen;
-                    mask |= (by_any ? 1u : 0u) << j;
-                    x[j] = seen ? x[j] : -INFINITY;
+                    x[j] = known && at + j >= lo && at + j < hi ? x[j] : -INFINITY;
                 }
             }
             float most = x[0];
@@ -644,29 +575,93 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, D <= 128 ? 2 : 1) void attn_deco
                 o[j] *= keep;
             }
         }
-        if (i + 1u < n) {
+        if (RING == 2 && i + 1u < n) {
             wait_fetches<FETCHES>(); // all but the next tile's keys
         } else {
             wait_fetches<0>();
         }
-        typename M::V v;
-        m.read_v(v, stage + BYTES, c, g);
-        if (whole) {
-            m.weigh(o, v, w, c);
-        } else {
-            M::clear(v, mask); // (a value that no row sees: 0 x infinity would be NaN)
-            if (RAGGED && __any(!M::finite(v))) {
-                m.weigh_finite(o, v, w, c, lo - at, known ? hi - at : 0);
-            } else {
-                m.weigh(o, v, w, c);
+        if (!whole) {
+            // What a row does not see must not reach it through a weight of zero: positions that
+            // no row sees become zeros (0 x infinity would be NaN), and so do values that are
+            // not finite where rows see different positions; those that see them are told
+            // after the loop.
+            const bool there = (PAGES == 1 || v_position < 16u ? now.id[0] : now.id[PAGES - 1]) < a.cache.pages;
+            const int from = there ? any_lo - (int)(base + v_position) : 0x7fffffff, upto = any_hi - (int)(base + v_position);
+            bool wrong = false;
+#pragma unroll 4
+            for (int f = 0; f < FETCHES; ++f) {
+                Unit *unit = (Unit *)(v_stage + f * 1024 + lane * 16u);
+                Unit v = *unit;
+#pragma unroll
+                for (int j = 0; j < VALUES; ++j) {
+                    const bool by_any = j >= from && j < upto, finite = !RAGGED || fabsf((float)v[j]) < INFINITY;
+                    wrong = wrong || (by_any && !finite);
+                    v[j] = by_any && finite ? v[j] : (T)0.0f;
+                }
+                *unit = v;
+            }
+            cleaned = cleaned || (RAGGED && __any(wrong));
+        }
+        {
+            const typename M::Weights p = M::pack(w, c);
+            auto read_v = [&](int t) { // channel 16 t + c, positions VALUES g and on
+                const uint32_t d = 16u * t + c;
+                return *(const Unit *)(v_stage + (d * 4u + (g ^ ((d >> 2) & 3u))) * 16u);
+            };
+            constexpr int AT_ONCE = PIECES < DT ? PIECES : DT;
+            Unit v[AT_ONCE], ahead[AT_ONCE];
+#pragma unroll
+            for (int t = 0; t < AT_ONCE; ++t) {
+                ahead[t] = read_v(t);
+            }
+#pragma unroll
+            for (int t0 = 0; t0 < DT; t0 += AT_ONCE) {
+#pragma unroll
+                for (int t = 0; t < AT_ONCE; ++t) {
+                    v[t] = ahead[t];
+                }
+                if (t0 + AT_ONCE < DT) {
+                    asm volatile("" ::: "memory");
+#pragma unroll
+                    for (int t = 0; t < AT_ONCE; ++t) {
+                        ahead[t] = read_v(t0 + AT_ONCE + t);
+                    }
+                } else if (RING == 1 && i + 1u < n) {
+                    wait_fetches<0>(); // (the reads of the values)
+                    fetch_k(i + 1u, next);
+                }
+#pragma unroll
+                for (int t = 0; t < AT_ONCE; ++t) {
+                    o[t0 + t] = M::weigh(o[t0 + t], v[t], p);
+                }
             }
         }
-        if (i + 1u < n) {
+        if (RING == 2 && i + 1u < n) {
             wait_fetches<FETCHES>(); // (the reads of the values)
             fetch_v(i + 1u, next);
         }
         now = next;
         next = after;
+    }
+
+    if (RAGGED && cleaned) {
+        // Rare, and as slow as it looks: every value of the wave's tiles that a row sees.
+        const int first = max(any_lo, (int)(start + TOKENS * t0)), last = min(any_hi, (int)(start + TOKENS * (t0 + n)));
+#pragma unroll 1
+        for (int at = first; at < last; ++at) {
+            const uint32_t page = table[min((uint32_t)at >> shift, last_entry)];
+            const bool seen = live && at >= lo && at < hi && page < a.cache.pages;
+            const T *v = (const T *)a.cache.v + head_page(page) + ((uint32_t)at & in_page);
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t d = 16u * t + 4u * g + j;
+                    const float x = (float)v[(FULL ? d : min(d, hd - 1u)) << shift];
+                    o[t][j] = seen && !(fabsf(x) < INFINITY) ? NAN : o[t][j];
+                }
+            }
+        }
     }
 
     // the waves' results

@@ -124,28 +124,14 @@ __device__ __forceinline__ void visible(const AttnArgs &a, int len, uint32_t seq
     hi = hi < len ? hi : len;
 }
 
-// A unit of values in two: what is finite, and 1 where it is not. Where rows of a tile see
-// different positions the first goes into the product with the weights (a weight of
-// zero would not keep an infinity or NaN from a row that does not see it), and the second
-// into a product with 1 for every position that a row sees, which counts the values
-// that make its result NaN.
-template <typename T, typename Unit, int E> __device__ __forceinline__ void part_finite(Unit &v, Unit &wrong) {
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-        const bool finite = fabsf((float)v[j]) < INFINITY;
-        wrong[j] = (T)(finite ? 0.0f : 1.0f);
-        v[j] = finite ? v[j] : (T)0.0f;
-    }
-}
-
 // Rows of sequence s0 + lane of a ragged batch, for a wave that goes through the sequences 64
-// at a time (`highest`: of the bounds before). A sequence has rows where its bounds ascend
+// at a time, and the first of them (`highest`: of the bounds before). A sequence has rows where its bounds ascend
 // within the batch and no earlier bound is above its first, so that no two sequences share
 // one.
-__device__ __forceinline__ uint32_t rows_of(const AttnArgs &a, uint32_t s0, uint32_t &highest) {
+__device__ __forceinline__ uint32_t rows_of(const AttnArgs &a, uint32_t s0, uint32_t &highest, uint32_t &first) {
     const uint32_t lane = threadIdx.x & 63u, s = min(s0 + lane, a.seqs - 1u);
     const uint32_t r0 = a.starts[s], r1 = a.starts[s + 1u];
-    uint32_t above = r0;
+    uint32_t above = first = r0;
     for (uint32_t x = 1; x < 64u; x <<= 1) {
         const uint32_t y = __shfl_up(above, x);
         above = lane >= x ? max(above, y) : above;
@@ -168,7 +154,8 @@ __device__ __forceinline__ uint32_t find_tile(const AttnArgs &a, uint32_t tile_r
         uint32_t before = 0, highest = 0;
         bool here = false;
         for (uint32_t s0 = 0; s0 < a.seqs && !here; s0 += 64u) {
-            const uint32_t n = rows_of(a, s0, highest) * a.group, mine = (n + tile_rows - 1u) / tile_rows;
+            uint32_t first;
+            const uint32_t n = rows_of(a, s0, highest, first) * a.group, mine = (n + tile_rows - 1u) / tile_rows;
             uint32_t upto = mine;
             for (uint32_t x = 1; x < 64u; x <<= 1) {
                 const uint32_t y = __shfl_up(upto, x);
@@ -180,7 +167,7 @@ __device__ __forceinline__ uint32_t find_tile(const AttnArgs &a, uint32_t tile_r
                     const int at = __builtin_ctzll(found);
                     seq = s0 + (uint32_t)at;
                     tile = want - before - (__shfl(upto, at) - __shfl(mine, at));
-                    row0 = a.starts[seq];
+                    row0 = __shfl(first, at);
                     rows = __shfl(n, at);
                     here = true;
                 }

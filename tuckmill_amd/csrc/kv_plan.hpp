@@ -10,10 +10,10 @@ namespace kv {
 // 16 columns of its matrix operand hold 8 heads in two f16 parts, or 16 in f32.
 inline uint32_t decode_cols(uint32_t type_id) { return type_id == 1u ? 8u : 16u; }
 
-// Shares of the positions: one for each CU. (In us, with 256, 512 and 1024 of them: a sequence
-// of 131071 tokens and 8 heads 100, 112, 130; 48 ragged ones up to 8192 156, 158, 155; 16 in
-// f32 with a window of 4096 30, 43, 52: the second workgroup of a CU starts late, and every
-// share is a part to join.)
+// Shares of the positions: one for each CU. (In us, with 256, 320 and 512 of them: a sequence
+// of 131071 tokens and 8 heads 101, 126, 111; 48 ragged ones up to 8192 156, 159, 157; 1500 f32
+// rows over a window 69, 69, 90; 256 f32 rows 17, 20, 20: the second workgroup of a CU
+// starts late, and every share is a part to join.)
 constexpr uint32_t DECODE_SHARES = 256;
 constexpr uint64_t DECODE_MAX_GRID = 1u << 23; // (a dimension of a grid is below 2^32 threads)
 constexpr uint32_t DECODE_WAVES = 4; // of a workgroup
@@ -61,7 +61,7 @@ constexpr uint64_t PREFILL_MAX_GROUPS = 1u << 23;
 // 2048 135 and 102; of 64 channels at 1024 50 and 60, at 2048 62 and 77; of 256 channels at
 // 2000 137 and 200, at 4000 500 and 357.) Pages of f32 it takes always: their products go at
 // a sixteenth of f16's rate, and its waves of 16 rows fill the card better than tiles of
-// 128 did (1500 rows of 256 channels 94 and 138, 4000 1250 and 1216, 4000 of 64 225 and 264).
+// 128 did (1500 rows of 256 channels 69 and 138, 4000 926 and 1216, 4000 of 128 347 and 509).
 constexpr uint64_t DECODE_MAX_UNITS = 1024;
 
 // Ragged rows. How they fall to sequences is known on the device only: every

@@ -57,7 +57,7 @@ hipError_t launch_lds(hipStream_t stream, hipEvent_t stop, dim3 grid, dim3 block
 template <typename T, int D, bool RAGGED>
 hipError_t launch_decode_as(hipStream_t stream, hipEvent_t stop, const kv::DecodeArgs &args, uint64_t grid_x) {
     const dim3 grid = args.shares != 0u ? dim3((uint32_t)grid_x) : dim3(args.a.cache.kv_heads * args.head_tiles, args.a.seqs);
-    constexpr uint32_t LDS = kv::DECODE_WAVES * 2u * 64u * D; // a tile's keys are 64 D bytes in either type
+    constexpr uint32_t LDS = kv::DecodeShape<T, D, RAGGED>::LDS;
     const dim3 block(64u * kv::DECODE_WAVES);
     return args.a.cache.head_dim == (uint32_t)D
                ? launch_lds<LDS, kv::attn_decode_kernel<T, D, true, RAGGED>>(stream, stop, grid, block, args)
