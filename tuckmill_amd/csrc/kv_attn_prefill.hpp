@@ -27,7 +27,9 @@ template <int D> struct PrefillShape {
     static constexpr int SWIZZLE = UK < 16 ? UK - 1 : 15;
 };
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 // How a row's q is held, the products and how weights enter the second one.
 template <int D, bool FULL> struct Rows {
@@ -81,13 +83,22 @@ template <int D, bool FULL> struct Rows {
         Unit hi[PIECES], lo[PIECES];
     };
     static __device__ __forceinline__ void pack(Weights &w, const float (&x)[S::SUB][16]) {
+        float minus = -1.0f;
+        asm("" : "+s"(minus));
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float y = x[i / 2][(i % 2) * 8 + j];
-                w.hi[i][j] = (_Float16)y;
-                w.lo[i][j] = (_Float16)(y - (float)w.hi[i][j]);
+            for (int j = 0; j < 8; j += 2) {
+                const float *y = &x[i / 2][(i % 2) * 8 + j];
+                const f16x2 hi = __builtin_convertvector((f32x2{y[0], y[1]}), f16x2);
+                // (y - hi, which is exact: one instruction that takes the f16 where it is, if the
+                // compiler does not know that `minus` is -1)
+                const f32x2 rest = {fmaf((float)hi[0], minus, y[0]), fmaf((float)hi[1], minus, y[1])};
+                const f16x2 lo = __builtin_convertvector(rest, f16x2);
+                w.hi[i][j] = hi[0];
+                w.hi[i][j + 1] = hi[1];
+                w.lo[i][j] = lo[0];
+                w.lo[i][j + 1] = lo[1];
             }
         }
     }
@@ -176,12 +187,6 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
     }
     const uint32_t s_begin = split * per, s_end = min(steps, s_begin + per);
 
-    R q;
-    const float unscale = q.load_q(a.q + (size_t)row * a.q_stride + (size_t)head * hd, h, hd, live);
-    const float slope = a.slopes != nullptr ? a.slopes[head] * LOG2E : 0.0f;
-    const float to_log2 = a.softcap > 0.0f ? a.scale * unscale / a.softcap : a.scale * unscale * LOG2E;
-    const float cap_log2 = a.softcap * LOG2E;
-
     // Pages of a step: one for every 16 positions.
     constexpr int PAGES = S::N / 16;
     const __attribute__((address_space(4))) uint32_t *table =
@@ -229,6 +234,16 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
         }
     };
 
+    if (s_begin < s_end) { // (on its way while the rows' q are taken apart)
+        look_up(s_begin);
+        fetch(s_begin, 0u);
+    }
+    R q;
+    const float unscale = q.load_q(a.q + (size_t)row * a.q_stride + (size_t)head * hd, h, hd, live);
+    const float slope = a.slopes != nullptr ? a.slopes[head] * LOG2E : 0.0f;
+    const float to_log2 = a.softcap > 0.0f ? a.scale * unscale / a.softcap : a.scale * unscale * LOG2E;
+    const float cap_log2 = a.softcap * LOG2E;
+
     f32x16 o[S::DT];
 #pragma unroll
     for (int t = 0; t < S::DT; ++t) {
@@ -238,10 +253,6 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
         }
     }
     float top = -3.402823466e38f, l = 0.0f;
-    if (s_begin < s_end) {
-        look_up(s_begin);
-        fetch(s_begin, 0u);
-    }
     for (uint32_t step = s_begin; step < s_end; ++step) {
 #pragma unroll
         for (int i = 0; i < PAGES; ++i) {
@@ -313,7 +324,20 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
                 cap_of(x[b], cap_log2);
             }
         }
-        if (a.slopes != nullptr) {
+        // Where a row sees no further than itself its bias is slope (position - p): a part that
+        // all of the lane's scores share (x is short of it, and so is what it is compared with)
+        // and one multiplication and addition each.
+        float shared = 0.0f;
+        if (a.slopes != nullptr && a.prefix == nullptr) {
+            shared = slope * (float)(mine - p);
+#pragma unroll
+            for (int b = 0; b < S::SUB; ++b) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    x[b][v] = fmaf(slope, (float)(32 * b + 16 * (v / 8) + v % 8), x[b][v]);
+                }
+            }
+        } else if (a.slopes != nullptr) {
 #pragma unroll
             for (int b = 0; b < S::SUB; ++b) {
 #pragma unroll
@@ -329,13 +353,14 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
         }
         const bool whole = known && base >= all_lo && base + S::N <= all_hi;
         if (!whole) {
+            const uint32_t first = (uint32_t)(lo - mine), count = lo < hi ? (uint32_t)(hi - lo) : 0u;
 #pragma unroll
-            for (int b = 0; b < S::SUB; ++b) {
+            for (int i = 0; i < PAGES; ++i) {
+                const uint32_t some = pages[i] < a.cache.pages ? count : 0u;
 #pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const int at = mine + 32 * b + 16 * (v / 8) + v % 8;
-                    const bool seen = at >= lo && at < hi && pages[2 * b + v / 8] < a.cache.pages;
-                    x[b][v] = seen ? x[b][v] : -INFINITY;
+                for (int v = 0; v < 8; ++v) {
+                    float &y = x[i / 2][8 * (i % 2) + v];
+                    y = 16u * i + v - first < some ? y : -INFINITY;
                 }
             }
         }
@@ -347,9 +372,10 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
                 most = fmaxf(most, x[b][v]);
             }
         }
-        if (__any(most > top + 8.0f)) {
+        if (__any(most + shared > top + 14.0f)) {
+            most = most + shared;
             most = fmaxf(most, __shfl_xor(most, 32));
-            most = fmaxf(most, top);
+            most = fmaxf(most - 6.0f, top);
             const float keep = exp2_of(top - most);
             top = most;
             l *= keep;
@@ -358,11 +384,12 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
                 o[t] *= keep;
             }
         }
+        const float reference = top - shared;
 #pragma unroll
         for (int b = 0; b < S::SUB; ++b) {
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
-                x[b][v] = exp2_of(x[b][v] - top + 6.0f);
+                x[b][v] = exp2_of(x[b][v] - reference);
                 l += x[b][v];
             }
         }

@@ -150,16 +150,19 @@ __device__ __forceinline__ uint32_t find_tile(const AttnArgs &a, uint32_t tile_r
     const uint32_t lane = threadIdx.x & 63u;
     uint32_t want = 0;
     seq = tile = row0 = rows = 0;
+    uint32_t first = 0, n = 0, mine = 0, upto = 0;
     for (int pass = 0; pass < 2; ++pass) {
         uint32_t before = 0, highest = 0;
         bool here = false;
         for (uint32_t s0 = 0; s0 < a.seqs && !here; s0 += 64u) {
-            uint32_t first;
-            const uint32_t n = rows_of(a, s0, highest, first) * a.group, mine = (n + tile_rows - 1u) / tile_rows;
-            uint32_t upto = mine;
-            for (uint32_t x = 1; x < 64u; x <<= 1) {
-                const uint32_t y = __shfl_up(upto, x);
-                upto += lane >= x ? y : 0u;
+            if (pass == 0 || a.seqs > 64u) {
+                n = rows_of(a, s0, highest, first) * a.group;
+                mine = (n + tile_rows - 1u) / tile_rows;
+                upto = mine;
+                for (uint32_t x = 1; x < 64u; x <<= 1) {
+                    const uint32_t y = __shfl_up(upto, x);
+                    upto += lane >= x ? y : 0u;
+                }
             }
             if (pass == 1) {
                 const uint64_t found = __ballot(want < before + upto);
