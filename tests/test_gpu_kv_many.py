@@ -194,3 +194,26 @@ def test_decode_scales_below_and_at_zero(ctx, type_id, scale, cap):
     got = run_decode(ctx, paged, q, 8, H.Attention(scale, cap))
     want, tol = want_decode(paged, q, 8, scale, softcap=cap)
     K.near(got, want, tol)
+
+
+@pytest.mark.parametrize("type_id", [K.F16, K.F32])
+@pytest.mark.parametrize("scattered", [0, 1])
+def test_of_rows_far_apart_that_name_one_slot_the_last_is_stored(ctx, type_id, scattered):
+    rng = np.random.default_rng(38)
+    tokens, heads, kv_heads, d, page = 2500, 2, 2, 16, 16
+    pages = 64
+    slots = rng.integers(0, pages * page, tokens) if scattered else np.arange(tokens) % (pages * page - 5)
+    q, k, v = (rng.standard_normal((tokens, h * d)).astype(np.float32) for h in (heads, kv_heads, kv_heads))
+    cache = H.KvCache.new(ctx, type_id, pages, page, kv_heads, d)
+    cache.k.upload(0, np.zeros((pages, kv_heads, page, d), K.DT[type_id]))
+    cache.v.upload(0, np.zeros((pages, kv_heads, d, page), K.DT[type_id]))
+    rope = H.Rope(upload_new(ctx, np.zeros(d // 2, np.float32)), d, [d // 2], False, False)  # (turns by nothing)
+    ctx.rope_store(rope, cache, *[upload_new(ctx, x) for x in (q, k, v)], ctx.buffer(q.nbytes),
+                   upload_new(ctx, K.u32(np.arange(tokens))), upload_new(ctx, K.u32(slots)), tokens, heads)
+    ctx.fence()
+    ek, ev = np.zeros((pages, kv_heads, page, d), K.DT[type_id]), np.zeros((pages, kv_heads, d, page), K.DT[type_id])
+    for t, s in enumerate(slots):
+        ek[s // page, :, s % page] = k[t].reshape(kv_heads, d)
+        ev[s // page, :, :, s % page] = v[t].reshape(kv_heads, d)
+    assert np.array_equal(cache.k.download(0, ek.nbytes).view(ek.dtype).reshape(ek.shape), ek)
+    assert np.array_equal(cache.v.download(0, ev.nbytes).view(ev.dtype).reshape(ev.shape), ev)

@@ -259,7 +259,7 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, 2) void attn_decode_kernel(Decod
     constexpr int PAGES = TOKENS / 16, KINDS = FETCHES / M::HALVES; // of lane offsets of keys
     // that a join takes at a time, of 8 bytes for each thread
     constexpr int PARTS = Shape::LDS / (8 * THREADS) < 32 ? Shape::LDS / (8 * THREADS) : 32;
-    extern __shared__ __align__(16) uint8_t lds[]; // keys and values of each wave; at the end the waves' results
+    extern __shared__ __align__(1024) uint8_t lds[]; // keys and values of each wave; at the end the waves' results
     static_assert(TOKENS * D * (int)sizeof(T) == BYTES && COLS == Shape::COLS, "results");
     float *merged = (float *)lds;
     __shared__ float stats[NW][2][COLS];

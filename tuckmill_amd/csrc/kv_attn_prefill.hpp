@@ -80,34 +80,29 @@ template <int D, bool FULL> struct Rows {
     }
     static constexpr int PIECES = S::N / 16; // of the weights: 16 positions each
     struct Weights {
-        Unit hi[PIECES], lo[PIECES];
+        Unit hi, lo;
     };
-    static __device__ __forceinline__ void pack(Weights &w, const float (&x)[S::SUB][16]) {
-        float minus = -1.0f;
-        asm("" : "+s"(minus));
+    static __device__ __forceinline__ Weights pack(const float (&x)[S::SUB][16], int i, float minus) {
+        Weights w;
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-                const float *y = &x[i / 2][(i % 2) * 8 + j];
-                const f16x2 hi = __builtin_convertvector((f32x2{y[0], y[1]}), f16x2);
-                // (y - hi, which is exact: one instruction that takes the f16 where it is, if the
-                // compiler does not know that `minus` is -1)
-                const f32x2 rest = {fmaf((float)hi[0], minus, y[0]), fmaf((float)hi[1], minus, y[1])};
-                const f16x2 lo = __builtin_convertvector(rest, f16x2);
-                w.hi[i][j] = hi[0];
-                w.hi[i][j + 1] = hi[1];
-                w.lo[i][j] = lo[0];
-                w.lo[i][j + 1] = lo[1];
-            }
+        for (int j = 0; j < 8; j += 2) {
+            const float *y = &x[i / 2][(i % 2) * 8 + j];
+            const f16x2 hi = __builtin_convertvector((f32x2{y[0], y[1]}), f16x2);
+            // (y - hi, which is exact: one instruction that takes the f16 where it is, if the
+            // compiler does not know that `minus` is -1)
+            const f32x2 rest = {fmaf((float)hi[0], minus, y[0]), fmaf((float)hi[1], minus, y[1])};
+            const f16x2 lo = __builtin_convertvector(rest, f16x2);
+            w.hi[j] = hi[0];
+            w.hi[j + 1] = hi[1];
+            w.lo[j] = lo[0];
+            w.lo[j + 1] = lo[1];
         }
+        return w;
     }
-    static __device__ __forceinline__ f32x16 weigh(f32x16 acc, const Unit &v, const Weights &w, int i) {
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w.hi[i], acc, 0, 0, 0);
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w.lo[i], acc, 0, 0, 0);
+    static __device__ __forceinline__ f32x16 weigh(f32x16 acc, const Unit &v, const Weights &w) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w.hi, acc, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w.lo, acc, 0, 0, 0);
     }
-    // unit of a channel's positions that piece i takes for lane half h
-    static __device__ __forceinline__ uint32_t v_unit(int i, uint32_t h) { return 2u * i + h; }
 };
 
 // A workgroup of four waves per key-value head, tile of 128 rows and share of the
@@ -119,20 +114,22 @@ template <int D, bool FULL> struct Rows {
 // In LDS the 16-byte units of a row are swapped by exclusive or with the row's number,
 // which spreads a column of units over the banks.
 // Bound by the matrix cores where rows are many: a prompt of 8192, 32 heads of 128 channels,
-// 1033 us = 532 TFLOP/s (1064 with both parts of q and of the weights counted); 4001 rows of packed
-// documents of 64 channels with bias and cap 62 us, bound by what happens to each score.
+// 980 us = 561 TFLOP/s (1122 with both parts of q and of the weights counted); 4001 rows of packed
+// documents of 64 channels with bias and cap 55 us, bound by what happens to each score and, at six
+// steps a workgroup, by how each begins and ends.
 template <int D, bool FULL, int WAVES_PER_SIMD>
 __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(PrefillArgs args) {
     typedef _Float16 T;
     typedef PrefillShape<D> S;
     typedef Rows<D, FULL> R;
     typedef typename R::Unit Unit;
-    extern __shared__ __align__(16) uint8_t lds[]; // two stages of keys and values
+    extern __shared__ __align__(1024) uint8_t lds[]; // two stages of keys and values
     __shared__ int range[4][2];
     __shared__ uint32_t arrived, cleaned;
     const AttnArgs &a = args.a;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t c = lane & 31u, h = lane >> 5;
+    const uint32_t stages = lds_address(lds); // (a multiple of a row of units)
     const uint32_t kvh = blockIdx.x % a.cache.kv_heads, rest = blockIdx.x / a.cache.kv_heads;
     const uint32_t split = rest % args.splits, index = rest / args.splits;
     const uint32_t hd = FULL ? (uint32_t)D : a.cache.head_dim, shift = a.cache.page_shift;
@@ -275,7 +272,6 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
         if (base >= any_hi || base + S::N <= any_lo) {
             continue; // nothing for this wave's rows
         }
-        uint8_t *k_lds = lds + stage * (2u * S::BYTES), *v_lds = k_lds + S::BYTES;
         f32x16 acc[S::SUB];
 #pragma unroll
         for (int b = 0; b < S::SUB; ++b) {
@@ -286,13 +282,18 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
         }
         // (each piece's reads stand before the products of the one in front of it and no
         // earlier: left alone, the compiler reads everything first and spills)
+        // A unit's address is its row's, with the bits of the unit that the lane and the piece
+        // give exchanged for one another's exclusive or: one instruction each, where addresses kept
+        // from step to step would take the registers of 16 bytes a lane for every piece.
+        typedef const __attribute__((address_space(3))) Unit *Lds;
+        const uint32_t k_at = stages + stage * (2u * S::BYTES) + (c * S::UK + (h ^ (c & S::SWIZZLE))) * 16u;
+        const uint32_t v_row = stages + stage * (2u * S::BYTES) + S::BYTES + (c * 8u + (h ^ (c & 7u))) * 16u;
         Unit k_next[S::SUB];
         auto read_k = [&](int s) {
 #pragma unroll
             for (int b = 0; b < S::SUB; ++b) {
-                const uint32_t at = 32u * b + c, unit = 2u * s + h;
-                const Unit k = *(const Unit *)(k_lds + (at * S::UK + (unit ^ (at & S::SWIZZLE))) * 16u);
-                k_next[b] = !FULL && unit * S::E >= hd ? Unit{} : k;
+                const Unit k = *(Lds)((k_at ^ (32u * s)) + b * (32u * S::UK * 16u));
+                k_next[b] = !FULL && (2u * s + h) * S::E >= hd ? Unit{} : k;
             }
         };
         read_k(0);
@@ -393,12 +394,9 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
                 l += x[b][v];
             }
         }
-        typename R::Weights w;
-        R::pack(w, x);
-        auto v_of = [&](int t, int i) {
-            const uint32_t d = 32u * t + c, unit = R::v_unit(i, h);
-            return (Unit *)(v_lds + (d * 8u + (unit ^ (d & 7u))) * 16u);
-        };
+        float minus = -1.0f;
+        asm("" : "+s"(minus));
+        auto v_of = [&](int t, int i) { return (v_row ^ (32u * i)) + t * (32u * 128u); };
         if (!whole) {
             // A value that is not finite must not reach a row that does not see it through
             // a weight of zero: it becomes zero in the stage (where the other waves may have
@@ -409,7 +407,7 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
 #pragma unroll
                 for (int i = 0; i < R::PIECES; ++i) {
                     asm volatile("" ::: "memory");
-                    bad = __builtin_elementwise_fma(*v_of(t, i), Unit{}, bad);
+                    bad = __builtin_elementwise_fma(*(Lds)v_of(t, i), Unit{}, bad);
                 }
             }
             bool any = false;
@@ -425,25 +423,29 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
                 for (int t = 0; t < S::DT; ++t) {
 #pragma unroll 1
                     for (int i = 0; i < R::PIECES; ++i) {
-                        Unit v = *v_of(t, i);
+                        Unit v = *(Lds)v_of(t, i);
 #pragma unroll
                         for (int j = 0; j < S::E; ++j) {
                             v[j] = fabsf((float)v[j]) < INFINITY ? v[j] : (T)0.0f;
                         }
-                        *v_of(t, i) = v;
+                        *(__attribute__((address_space(3))) Unit *)v_of(t, i) = v;
                     }
                 }
             }
         }
-        Unit v_next = *v_of(0, 0);
+        Unit v_next = *(Lds)v_of(0, 0);
 #pragma unroll
-        for (int i = 0; i < R::PIECES * S::DT; ++i) {
-            const Unit v = v_next;
-            asm volatile("" ::: "memory");
-            if (i + 1 < R::PIECES * S::DT) {
-                v_next = *v_of((i + 1) % S::DT, (i + 1) / S::DT);
+        for (int i = 0; i < R::PIECES; ++i) {
+            const typename R::Weights w = R::pack(x, i, minus);
+#pragma unroll
+            for (int t = 0; t < S::DT; ++t) {
+                const Unit v = v_next;
+                asm volatile("" ::: "memory");
+                if (i * S::DT + t + 1 < R::PIECES * S::DT) {
+                    v_next = *(Lds)v_of((t + 1) % S::DT, i + (t + 1) / S::DT);
+                }
+                o[t] = R::weigh(o[t], v, w);
             }
-            o[i % S::DT] = R::weigh(o[i % S::DT], v, w, i / S::DT);
         }
     }
     l += __shfl_xor(l, 32);

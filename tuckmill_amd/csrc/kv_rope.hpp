@@ -62,16 +62,29 @@ template <typename T, bool WIDE> __global__ __launch_bounds__(256) void rope_sto
             slot_of[threadIdx.x] = (slot >> a.page_shift) < a.pages ? slot : 0xffffffffu;
         }
         __syncthreads();
-        uint32_t mine[ROPE_ROWS], again = 0;
+        // (each later row is compared with all of these only if it lies between them)
+        uint32_t mine[ROPE_ROWS], lowest = 0xffffffffu, highest = 0, again = 0;
 #pragma unroll
         for (uint32_t r = 0; r < ROPE_ROWS; ++r) {
             mine[r] = slot_of[r];
+            lowest = min(lowest, mine[r]);
+            highest = mine[r] != 0xffffffffu ? max(highest, mine[r]) : highest;
         }
-        for (uint32_t u = t0 + 1u + threadIdx.x; u < a.tokens; u += 256u) {
-            const uint32_t other = a.slots[u];
+        for (uint32_t u0 = t0 + 1u + threadIdx.x; u0 < a.tokens; u0 += 4u * 256u) {
+            uint32_t other[4];
 #pragma unroll
-            for (uint32_t r = 0; r < ROPE_ROWS; ++r) {
-                again |= other == mine[r] && u > t0 + r ? 1u << r : 0u;
+            for (uint32_t k = 0; k < 4u; ++k) {
+                other[k] = a.slots[min(u0 + 256u * k, a.tokens - 1u)];
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k) {
+                const uint32_t u = min(u0 + 256u * k, a.tokens - 1u);
+                if (other[k] >= lowest && other[k] <= highest) {
+#pragma unroll
+                    for (uint32_t r = 0; r < ROPE_ROWS; ++r) {
+                        again |= other[k] == mine[r] && u > t0 + r ? 1u << r : 0u;
+                    }
+                }
             }
         }
         __syncthreads();
