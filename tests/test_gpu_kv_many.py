@@ -217,3 +217,25 @@ def test_of_rows_far_apart_that_name_one_slot_the_last_is_stored(ctx, type_id, s
         ev[s // page, :, :, s % page] = v[t].reshape(kv_heads, d)
     assert np.array_equal(cache.k.download(0, ek.nbytes).view(ek.dtype).reshape(ek.shape), ek)
     assert np.array_equal(cache.v.download(0, ev.nbytes).view(ev.dtype).reshape(ev.shape), ev)
+
+
+@pytest.mark.parametrize("type_id,heads,kv_heads", [(K.F16, 8, 4), (K.F32, 8, 4), (K.F16, 64, 64)])
+@pytest.mark.parametrize("cap", [0.0, 2.0 ** -140])
+def test_steep_biases_and_a_cap_of_next_to_nothing(ctx, type_id, heads, kv_heads, cap):
+    rng = np.random.default_rng(39)
+    news, lens = [130, 6], [230, 40]
+    paged = K.Paged(rng, type_id, 16, kv_heads, 64, lens)
+    paged.keys[0][100] = 0  # scores of zero
+    paged.put(0, 100)
+    starts, _, _ = prefill_case(rng, news, lens)
+    q = rng.standard_normal((136, heads * 64)).astype(np.float32)
+    slopes = (2.0 ** rng.integers(-3, 6, heads) * 1.1).astype(np.float32)
+    attn = H.Attention(0.125, cap, slopes=upload_new(ctx, slopes))
+    got = run_prefill(ctx, paged, q, heads, attn, starts)
+    want, tol = want_prefill(paged, q, heads, starts, news, 0.125, softcap=cap, slopes=slopes)
+    K.near(got, want, tol)
+    if many(136, 2, heads, kv_heads):
+        return
+    got = run_decode(ctx, paged, q[:2], heads, attn)
+    want, tol = want_decode(paged, q[:2], heads, 0.125, softcap=cap, slopes=slopes)
+    K.near(got, want, tol)

@@ -467,7 +467,7 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, 2) void attn_decode_kernel(Decod
                                    a.scale < 0.0f ? -1.0f : 1.0f);
     const float slope = a.slopes != nullptr ? a.slopes[head] * LOG2E : 0.0f;
     const float scale = fabsf(a.scale) * unscale; // (its sign is with q)
-    const float to_log2 = a.softcap > 0.0f ? scale / a.softcap : scale * LOG2E;
+    const float to_log2 = score_factor(scale, a.softcap);
     const float cap_log2 = a.softcap * LOG2E;
 
     f32x4 o[DT];
@@ -538,7 +538,7 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, 2) void attn_decode_kernel(Decod
             if (a.slopes != nullptr) {
 #pragma unroll
                 for (int j = 0; j < VALUES; ++j) {
-                    x[j] -= slope * fabsf((float)(p - at - j));
+                    x[j] = fmaf(-slope, fabsf((float)(at - p) + (float)j), x[j]);
                 }
             }
             if (!whole) {

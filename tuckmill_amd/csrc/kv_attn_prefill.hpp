@@ -238,7 +238,7 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
     R q;
     const float unscale = q.load_q(a.q + (size_t)row * a.q_stride + (size_t)head * hd, h, hd, live);
     const float slope = a.slopes != nullptr ? a.slopes[head] * LOG2E : 0.0f;
-    const float to_log2 = a.softcap > 0.0f ? a.scale * unscale / a.softcap : a.scale * unscale * LOG2E;
+    const float to_log2 = score_factor(a.scale * unscale, a.softcap);
     const float cap_log2 = a.softcap * LOG2E;
 
     f32x16 o[S::DT];
@@ -325,25 +325,13 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
                 cap_of(x[b], cap_log2);
             }
         }
-        // Where a row sees no further than itself its bias is slope (position - p): a part that
-        // all of the lane's scores share (x is short of it, and so is what it is compared with)
-        // and one multiplication and addition each.
-        float shared = 0.0f;
-        if (a.slopes != nullptr && a.prefix == nullptr) {
-            shared = slope * (float)(mine - p);
+        if (a.slopes != nullptr) {
+            const float from = (float)(mine - p);
 #pragma unroll
             for (int b = 0; b < S::SUB; ++b) {
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
-                    x[b][v] = fmaf(slope, (float)(32 * b + 16 * (v / 8) + v % 8), x[b][v]);
-                }
-            }
-        } else if (a.slopes != nullptr) {
-#pragma unroll
-            for (int b = 0; b < S::SUB; ++b) {
-#pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    x[b][v] -= slope * fabsf((float)(p - mine - (32 * b + 16 * (v / 8) + v % 8)));
+                    x[b][v] = fmaf(-slope, fabsf(from + (float)(32 * b + 16 * (v / 8) + v % 8)), x[b][v]);
                 }
             }
         }
@@ -373,8 +361,7 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
                 most = fmaxf(most, x[b][v]);
             }
         }
-        if (__any(most + shared > top + 14.0f)) {
-            most = most + shared;
+        if (__any(most > top + 14.0f)) {
             most = fmaxf(most, __shfl_xor(most, 32));
             most = fmaxf(most - 6.0f, top);
             const float keep = exp2_of(top - most);
@@ -385,12 +372,11 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
                 o[t] *= keep;
             }
         }
-        const float reference = top - shared;
 #pragma unroll
         for (int b = 0; b < S::SUB; ++b) {
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
-                x[b][v] = exp2_of(x[b][v] - reference);
+                x[b][v] = exp2_of(x[b][v] - top);
                 l += x[b][v];
             }
         }

@@ -64,6 +64,13 @@ template <int N> __device__ __forceinline__ void cap_of(float (&x)[N], float cap
     }
 }
 
+// What a dot product is multiplied by: to a score in units of the cap, or of log2 e. (Finite for
+// a cap of next to nothing too, or a dot product of zero would become NaN.)
+__device__ __forceinline__ float score_factor(float scale, float cap) {
+    const float by = cap > 0.0f ? scale / cap : scale * LOG2E;
+    return __builtin_amdgcn_fmed3f(by, -3.402823466e38f, 3.402823466e38f);
+}
+
 // The power of two that brings a largest magnitude to about 2^13 (none where it is not
 // finite), at which two f16 parts hold 22 bits of it without overflow.
 __device__ __forceinline__ int scale_bits(float top) {
