@@ -239,3 +239,26 @@ def test_steep_biases_and_a_cap_of_next_to_nothing(ctx, type_id, heads, kv_heads
     got = run_decode(ctx, paged, q[:2], heads, attn)
     want, tol = want_decode(paged, q[:2], heads, 0.125, softcap=cap, slopes=slopes)
     K.near(got, want, tol)
+
+
+@pytest.mark.parametrize("rows,vocab", [(3, 3000), (40, 60001)])
+@pytest.mark.parametrize("hist,biases", [(65535, 65534), (65536, 5), (5, 65535), (70000, 70000)])
+def test_logits_with_long_lists(ctx, rows, vocab, hist, biases):
+    rng = np.random.default_rng(40)
+    x = (rng.standard_normal((rows, vocab)) * 5).astype(np.float32)
+    history = rng.integers(0, vocab + 3, (rows, hist)).astype(np.uint32)
+    history[0] = 7  # one id, as often as there are entries
+    ids = rng.integers(0, vocab + 3, (rows, biases)).astype(np.uint32)
+    ids[1] = 8  # one id: the last entry counts
+    values = rng.standard_normal((rows, biases)).astype(np.float32)
+    hl, bl = np.full(rows, hist + 9), np.full(rows, biases)
+    hl[2], bl[2] = hist // 2, biases // 2
+    pen = np.tile(np.array([1.3, 0.4, 1e-3], np.float32), (rows, 1))
+    bufs = [upload_new(ctx, v) for v in (history, K.u32(hl), pen, ids, values, K.u32(bl))]
+    adjust = H.LogitsAdjust(*bufs, history_stride=hist, bias_stride=biases)
+    xb = upload_new(ctx, x)
+    out = ctx.buffer(x.nbytes)
+    ctx.logits_adjust(adjust, xb, out, rows, vocab)
+    ctx.fence()
+    want, tol = K.adjust(x, history, hl, pen, ids, values, bl)
+    K.near(f32(out, x.shape), want, tol)

@@ -313,7 +313,7 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, 2) void attn_decode_kernel(Decod
         auto add_up = [&]() {
             const uint64_t shares = size != 0u ? (steps_here + size - 1u) / size : 0u;
             upto = (uint64_t)units_of(rows_here) * (size == 0u ? steps_here : shares > 1u ? shares | shares << 32 : shares);
-            for (uint32_t x = 1; x < 64u; x <<= 1) {
+            for (uint32_t x = 1; x <= last_lane(a); x <<= 1) {
                 const uint64_t y = __shfl_up(upto, x);
                 upto += lane >= x ? y : 0u;
             }
@@ -328,7 +328,7 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, 2) void attn_decode_kernel(Decod
             add_up();
         };
         auto look_on = [&]() {
-            before += __shfl(upto, 63);
+            before += __shfl(upto, last_lane(a));
             highest = rows_up_to;
             s0 += 64u;
             look();
@@ -337,7 +337,7 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, 2) void attn_decode_kernel(Decod
         while (s0 + 64u < a.seqs) {
             look_on();
         }
-        size = (uint32_t)((before + __shfl(upto, 63) + args.shares - 1u) / args.shares);
+        size = (uint32_t)((before + __shfl(upto, last_lane(a)) + args.shares - 1u) / args.shares);
         size = __builtin_amdgcn_readfirstlane(max(size, 1u));
         before = 0;
         if (s0 == 0u) {
@@ -386,12 +386,10 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, 2) void attn_decode_kernel(Decod
     visible(a, len, seq, row0 + query, p, lo, hi);
     int any_lo = lo < hi ? lo : 0x7fffffff, any_hi = lo < hi ? hi : 0, all_lo = lo, all_hi = hi;
     if constexpr (RAGGED) {
-        for (int x = 8; x > 0; x >>= 1) {
-            any_lo = min(any_lo, __shfl_xor(any_lo, x));
-            any_hi = max(any_hi, __shfl_xor(any_hi, x));
-            all_lo = max(all_lo, __shfl_xor(all_lo, x));
-            all_hi = min(all_hi, __shfl_xor(all_hi, x));
-        }
+        any_lo = least16(any_lo);
+        any_hi = most16(any_hi);
+        all_lo = most16(all_lo);
+        all_hi = least16(all_hi);
     }
     any_lo = __builtin_amdgcn_readfirstlane(any_lo);
     any_hi = __builtin_amdgcn_readfirstlane(any_hi);

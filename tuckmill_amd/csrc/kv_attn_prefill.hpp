@@ -155,16 +155,10 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
     // there may be given anything.)
     const bool sees = live && lo < hi;
     int any_lo = sees ? lo : 0x7fffffff, any_hi = sees ? hi : 0, all_lo = live ? lo : 0, all_hi = live ? hi : 0x7fffffff;
-    for (int x = 32; x > 0; x >>= 1) {
-        any_lo = min(any_lo, __shfl_xor(any_lo, x));
-        any_hi = max(any_hi, __shfl_xor(any_hi, x));
-        all_lo = max(all_lo, __shfl_xor(all_lo, x));
-        all_hi = min(all_hi, __shfl_xor(all_hi, x));
-    }
-    any_lo = __builtin_amdgcn_readfirstlane(any_lo);
-    any_hi = __builtin_amdgcn_readfirstlane(any_hi);
-    all_lo = __builtin_amdgcn_readfirstlane(all_lo);
-    all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+    any_lo = least64(any_lo);
+    any_hi = most64(any_hi);
+    all_lo = most64(all_lo);
+    all_hi = least64(all_hi);
     if (threadIdx.x == 0u) {
         cleaned = 0u;
     }

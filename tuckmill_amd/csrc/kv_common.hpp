@@ -131,6 +131,37 @@ __device__ __forceinline__ void visible(const AttnArgs &a, int len, uint32_t seq
     hi = hi < len ? hi : len;
 }
 
+// The smallest and the largest of a row of 16 lanes, in all of them; and of the wave, as a scalar.
+template <int N> __device__ __forceinline__ int ror(int x) {
+    return __builtin_amdgcn_update_dpp(0, x, 0x120 + N, 0xf, 0xf, false);
+}
+__device__ __forceinline__ int least16(int x) {
+    x = min(x, ror<8>(x));
+    x = min(x, ror<4>(x));
+    x = min(x, ror<2>(x));
+    return min(x, ror<1>(x));
+}
+__device__ __forceinline__ int most16(int x) {
+    x = max(x, ror<8>(x));
+    x = max(x, ror<4>(x));
+    x = max(x, ror<2>(x));
+    return max(x, ror<1>(x));
+}
+__device__ __forceinline__ int least64(int x) {
+    x = least16(x);
+    return min(min(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16)),
+               min(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48)));
+}
+__device__ __forceinline__ int most64(int x) {
+    x = most16(x);
+    return max(max(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16)),
+               max(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48)));
+}
+
+// The last lane of a wave that goes through the sequences, one a lane: sums and maxima over the lanes
+// before each stop there (a few sequences need few steps).
+__device__ __forceinline__ uint32_t last_lane(const AttnArgs &a) { return min(a.seqs, 64u) - 1u; }
+
 // Rows of sequence s0 + lane of a ragged batch, for a wave that goes through the sequences 64
 // at a time, and the first of them (`highest`: of the bounds before). A sequence has rows where its bounds ascend
 // within the batch and no earlier bound is above its first, so that no two sequences share
@@ -139,12 +170,12 @@ __device__ __forceinline__ uint32_t rows_of(const AttnArgs &a, uint32_t s0, uint
     const uint32_t lane = threadIdx.x & 63u, s = min(s0 + lane, a.seqs - 1u);
     const uint32_t r0 = a.starts[s], r1 = a.starts[s + 1u];
     uint32_t above = first = r0;
-    for (uint32_t x = 1; x < 64u; x <<= 1) {
+    for (uint32_t x = 1; x <= last_lane(a); x <<= 1) {
         const uint32_t y = __shfl_up(above, x);
         above = lane >= x ? max(above, y) : above;
     }
     above = max(above, highest);
-    highest = __shfl(above, 63);
+    highest = __shfl(above, last_lane(a));
     return s0 + lane < a.seqs && r0 == above && r0 <= r1 && r1 <= a.tokens ? r1 - r0 : 0u;
 }
 
@@ -166,7 +197,7 @@ __device__ __forceinline__ uint32_t find_tile(const AttnArgs &a, uint32_t tile_r
                 n = rows_of(a, s0, highest, first) * a.group;
                 mine = (n + tile_rows - 1u) / tile_rows;
                 upto = mine;
-                for (uint32_t x = 1; x < 64u; x <<= 1) {
+                for (uint32_t x = 1; x <= last_lane(a); x <<= 1) {
                     const uint32_t y = __shfl_up(upto, x);
                     upto += lane >= x ? y : 0u;
                 }
@@ -182,7 +213,7 @@ __device__ __forceinline__ uint32_t find_tile(const AttnArgs &a, uint32_t tile_r
                     here = true;
                 }
             }
-            before += __shfl(upto, 63);
+            before += __shfl(upto, last_lane(a));
         }
         if (pass == 0) {
             if (index >= before) {

@@ -24,11 +24,14 @@ struct LogitsArgs {
 // stream of logits where there are many rows: every tile reads the lists again, so
 // tiles are large there; a single row is a matter of latency, and small tiles
 // spread it over the card.
-template <int TILE, int THREADS>
+// SHORT: lists of fewer than 2^16 entries, whose counts and indices share a word: four workgroups of
+// a large tile on a CU instead of two.
+template <int TILE, int THREADS, bool SHORT>
 __global__ __launch_bounds__(THREADS) void logits_adjust_kernel(LogitsArgs a) {
     constexpr int PER = TILE / THREADS; // logits of a thread, in pieces of four
     __shared__ __align__(16) uint32_t count[TILE];
-    __shared__ __align__(16) uint32_t entry[TILE]; // 1 + its index, 0: none
+    __shared__ __align__(16) uint32_t entries[SHORT ? 4 : TILE];
+    uint32_t *entry = SHORT ? count : entries; // 1 + its index, 0: none (SHORT: in the upper half)
     const uint32_t row = blockIdx.y, id0 = blockIdx.x * TILE;
     const uint32_t here = min((uint32_t)TILE, a.vocab - id0);
     const float *x = a.x + (size_t)row * a.vocab + id0;
@@ -59,15 +62,30 @@ __global__ __launch_bounds__(THREADS) void logits_adjust_kernel(LogitsArgs a) {
         for (int j = 0; j < PER / 4; ++j) {
             const uint32_t at = threadIdx.x + (uint32_t)(j * THREADS);
             ((q8::u32x4 *)count)[at] = q8::u32x4{0u, 0u, 0u, 0u};
-            ((q8::u32x4 *)entry)[at] = q8::u32x4{0u, 0u, 0u, 0u};
+            if constexpr (!SHORT) {
+                ((q8::u32x4 *)entries)[at] = q8::u32x4{0u, 0u, 0u, 0u};
+            }
         }
         __syncthreads();
+        if (a.bias_ids != nullptr) { // (first: the largest index is found while the counts are zero)
+            const uint32_t n = min(a.bias_len[row], a.bias_stride);
+            const uint32_t *ids = a.bias_ids + (size_t)row * a.bias_stride;
+            for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+                const uint32_t at = ids[i] - id0; // (below id0 wraps to a large value)
+                if (at < (uint32_t)TILE) {
+                    atomicMax(&entry[at], SHORT ? (i + 1u) << 16 : i + 1u);
+                }
+            }
+            if (SHORT && a.history != nullptr) {
+                __syncthreads();
+            }
+        }
         if (a.history != nullptr) {
             const uint32_t n = min(a.history_len[row], a.history_stride);
             const uint32_t *ids = a.history + (size_t)row * a.history_stride;
 #pragma unroll 4
             for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-                const uint32_t at = ids[i] - id0; // (below id0 wraps to a large value)
+                const uint32_t at = ids[i] - id0;
                 if (at < (uint32_t)TILE) {
                     atomicAdd(&count[at], 1u);
                 }
@@ -75,16 +93,6 @@ __global__ __launch_bounds__(THREADS) void logits_adjust_kernel(LogitsArgs a) {
             rep = a.penalties[(size_t)row * 3u];
             presence = a.penalties[(size_t)row * 3u + 1u];
             frequency = a.penalties[(size_t)row * 3u + 2u];
-        }
-        if (a.bias_ids != nullptr) {
-            const uint32_t n = min(a.bias_len[row], a.bias_stride);
-            const uint32_t *ids = a.bias_ids + (size_t)row * a.bias_stride;
-            for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-                const uint32_t at = ids[i] - id0;
-                if (at < (uint32_t)TILE) {
-                    atomicMax(&entry[at], i + 1u);
-                }
-            }
         }
         __syncthreads();
     }
@@ -97,7 +105,11 @@ __global__ __launch_bounds__(THREADS) void logits_adjust_kernel(LogitsArgs a) {
             allowed = a.allowed[(size_t)row * a.allowed_stride + (id >> 5)] >> (id & 31u);
         }
         if (listed) {
-            const q8::u32x4 c = ((const q8::u32x4 *)count)[at / 4u], e = ((const q8::u32x4 *)entry)[at / 4u];
+            q8::u32x4 c = ((const q8::u32x4 *)count)[at / 4u], e = ((const q8::u32x4 *)entry)[at / 4u];
+            if constexpr (SHORT) {
+                c &= 0xffffu;
+                e >>= 16;
+            }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 float z = v[4 * j + k];

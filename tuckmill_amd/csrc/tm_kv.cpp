@@ -170,12 +170,21 @@ hipError_t launch_logits(hipStream_t stream, hipEvent_t stop, const Op &op) {
     a.bias_stride = p.bias_stride;
     a.allowed_stride = p.allowed_stride;
     auto tiles = [&](uint64_t tile) { return (uint32_t)((op.cols + tile - 1u) / tile); };
+    const bool is_short = p.history_stride < 65536u && p.bias_stride < 65535u;
     if ((uint64_t)tiles(kv::LOGITS_LARGE) * op.rows >= kv::LOGITS_MIN_GROUPS) {
-        Q8_LAUNCH((kv::logits_adjust_kernel<kv::LOGITS_LARGE, 512>), dim3(tiles(kv::LOGITS_LARGE), op.rows), dim3(512), 0,
-                  stream, stop, a);
+        const dim3 grid(tiles(kv::LOGITS_LARGE), op.rows);
+        if (is_short) {
+            Q8_LAUNCH((kv::logits_adjust_kernel<kv::LOGITS_LARGE, 512, true>), grid, dim3(512), 0, stream, stop, a);
+        } else {
+            Q8_LAUNCH((kv::logits_adjust_kernel<kv::LOGITS_LARGE, 512, false>), grid, dim3(512), 0, stream, stop, a);
+        }
     } else {
-        Q8_LAUNCH((kv::logits_adjust_kernel<kv::LOGITS_SMALL, 256>), dim3(tiles(kv::LOGITS_SMALL), op.rows), dim3(256), 0,
-                  stream, stop, a);
+        const dim3 grid(tiles(kv::LOGITS_SMALL), op.rows);
+        if (is_short) {
+            Q8_LAUNCH((kv::logits_adjust_kernel<kv::LOGITS_SMALL, 256, true>), grid, dim3(256), 0, stream, stop, a);
+        } else {
+            Q8_LAUNCH((kv::logits_adjust_kernel<kv::LOGITS_SMALL, 256, false>), grid, dim3(256), 0, stream, stop, a);
+        }
     }
     return hipGetLastError();
 }
