@@ -1,5 +1,5 @@
 """Paged attention where a call has many rows, many sequences or long ones: ragged batches
-of f16 pages with enough rows for the kernel with tiles of 128 (more than 1024 tiles of eight
+of f16 pages with enough rows for the kernel with tiles of 128 (more than 1056 tiles of eight
 rows over all key-value heads), and the shares that the other kernel cuts positions into."""
 import numpy as np
 import pytest
@@ -22,7 +22,7 @@ def ctx():
 
 def many(rows, seqs, heads, kv_heads):
     """Whether the rows are enough for tiles of 128."""
-    return (rows * (heads // kv_heads) // 8 + seqs) * kv_heads > 1024
+    return (rows * (heads // kv_heads) // 8 + seqs) * kv_heads > 1056
 
 
 @pytest.mark.parametrize("heads,kv_heads,d,page", [

@@ -126,6 +126,7 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
     extern __shared__ __align__(1024) uint8_t lds[]; // two stages of keys and values
     __shared__ int range[4][2];
     __shared__ uint32_t arrived, cleaned;
+    __shared__ float factor[PREFILL_MAX_SPLITS][128];
     const AttnArgs &a = args.a;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t c = lane & 31u, h = lane >> 5;
@@ -171,8 +172,8 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
     const int upto = max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1]));
     const uint32_t start = __builtin_amdgcn_readfirstlane(from < upto ? (uint32_t)from & ~(uint32_t)(S::N - 1) : 0u);
     const uint32_t steps = __builtin_amdgcn_readfirstlane(from < upto ? ((uint32_t)upto - start + S::N - 1u) / S::N : 0u);
-    const uint32_t per = (steps + args.splits - 1u) / args.splits;
-    const uint32_t parts = per != 0u ? (steps + per - 1u) / per : 1u;
+    const uint32_t shares = max(min(args.splits, steps / PREFILL_MIN_STEPS), 1u), per = (steps + shares - 1u) / shares;
+    const uint32_t parts = steps != 0u ? (steps + per - 1u) / per : 1u;
     if (split >= parts) {
         return;
     }
@@ -485,23 +486,28 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
     const size_t part_floats = 128u * (size_t)(hd + 2u);
     const size_t slot = (size_t)want * a.cache.kv_heads + kvh;
     const float *first = args.partials + slot * args.splits * part_floats;
+    const uint32_t here = min(128u, rows - tile * 128u), pairs = hd / 2u;
+    // (by way of LDS, so that a wave's stores lie side by side; units swapped as in a stage)
+    float *all = (float *)lds;
+    static_assert(4 * S::BYTES == 128 * D * 4, "results");
+#pragma unroll
+    for (int t = 0; t < S::DT; ++t) {
+#pragma unroll
+        for (int v = 0; v < 16; v += 4) {
+            const uint32_t at = wave * 32u + c, unit = 8u * t + v / 2u + h;
+            *(f32x4 *)(all + at * D + (unit ^ (c & 15u)) * 4u) = f32x4{o[t][v], o[t][v + 1], o[t][v + 2], o[t][v + 3]};
+        }
+    }
+    __syncthreads();
     {
         float *to = (float *)first + split * part_floats;
-        const uint32_t at = wave * 32u + c;
-        if (live) {
-#pragma unroll
-            for (int t = 0; t < S::DT; ++t) {
-#pragma unroll
-                for (int v = 0; v < 16; v += 2) {
-                    const uint32_t d = 32u * t + 8u * (v / 4) + 4u * h + (v % 4);
-                    if (FULL || d < hd) {
-                        put2(to + at * hd + d, o[t][v], o[t][v + 1]);
-                    }
-                }
-            }
-            if (h == 0u) {
-                put2(to + 128u * hd + 2u * at, top, l);
-            }
+        for (uint32_t i = threadIdx.x; i < here * pairs; i += 256u) {
+            const uint32_t at = i / pairs, d = 2u * (i % pairs);
+            const float *from = all + at * D + ((d >> 2) ^ (at & 15u)) * 4u + (d & 2u);
+            put2(to + 2u * i, from[0], from[1]);
+        }
+        if (live && h == 0u) {
+            put2(to + 128u * hd + 2u * (wave * 32u + c), top, l);
         }
     }
     __builtin_amdgcn_s_waitcnt(7 << 4);
@@ -518,44 +524,59 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
     if (threadIdx.x == 0u) {
         __hip_atomic_store(&args.arrivals[slot], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    const uint32_t here = min(128u, rows - tile * 128u);
-    float *factor = (float *)lds; // [row][part], then 128 sums
-    float *sums = factor + 128u * PREFILL_MAX_SPLITS;
+    // Weights of the parts, then as many rows at a time as LDS holds of all parts: every load is
+    // a trip past the L2, so all of a turn's are on their way at once.
     if (threadIdx.x < here) {
         const float *stats = first + 128u * hd + 2u * threadIdx.x;
-        float best = -3.402823466e38f, sum = 0.0f;
-        for (uint32_t s = 0; s < parts; ++s) {
-            float t, y;
-            get2(stats + s * part_floats, t, y);
-            best = fmaxf(best, t);
+        float t[PREFILL_MAX_SPLITS], y[PREFILL_MAX_SPLITS];
+#pragma unroll
+        for (uint32_t s = 0; s < PREFILL_MAX_SPLITS; ++s) {
+            t[s] = -INFINITY;
+            y[s] = 0.0f;
+            if (s < parts) {
+                get2(stats + s * part_floats, t[s], y[s]);
+            }
         }
-        for (uint32_t s = 0; s < parts; ++s) {
-            float t, y;
-            get2(stats + s * part_floats, t, y);
-            const float f = exp2_of(t - best);
-            factor[threadIdx.x * PREFILL_MAX_SPLITS + s] = f;
-            sum += f * y;
+        float best = t[0], sum = 0.0f;
+#pragma unroll
+        for (uint32_t s = 1; s < PREFILL_MAX_SPLITS; ++s) {
+            best = fmaxf(best, t[s]);
         }
-        sums[threadIdx.x] = sum;
+#pragma unroll
+        for (uint32_t s = 0; s < PREFILL_MAX_SPLITS; ++s) {
+            t[s] = exp2_of(t[s] - best);
+            sum += t[s] * y[s];
+        }
+#pragma unroll
+        for (uint32_t s = 0; s < PREFILL_MAX_SPLITS; ++s) {
+            factor[s][threadIdx.x] = sum == 0.0f ? 0.0f : t[s] / sum;
+        }
     }
-    __syncthreads();
-    const uint32_t pairs = hd / 2u;
-    for (uint32_t i = threadIdx.x; i < here * pairs; i += 256u) {
-        const uint32_t at = i / pairs, d = 2u * (i % pairs);
-        float y0 = 0.0f, y1 = 0.0f;
-#pragma unroll 4
-        for (uint32_t s = 0; s < parts; ++s) {
-            float u0, u1;
-            get2(first + s * part_floats + at * hd + d, u0, u1);
-            const float f = factor[at * PREFILL_MAX_SPLITS + s];
-            y0 += f * u0;
-            y1 += f * u1;
+    const uint32_t row_bytes = hd * 4u;
+    const uint32_t at_once = 4u * S::BYTES / 1024u / parts * 1024u / row_bytes; // (pieces of 1 KiB of each part)
+    for (uint32_t r0 = 0; r0 < here; r0 += at_once) {
+        const uint32_t some = min(at_once, here - r0), bytes = some * row_bytes, pieces = (bytes + 1023u) / 1024u;
+        __syncthreads(); // (what lay there has been read, the factors have been written)
+        for (uint32_t f = wave; f < parts * pieces; f += 4u) {
+            const uint8_t *part = (const uint8_t *)(first + (f / pieces) * part_floats + r0 * hd);
+            fetch16_past(part + min((f % pieces) * 1024u + lane * 16u, bytes - 16u), stages + f * 1024u);
         }
-        const uint32_t rr = tile * 128u + at;
-        const float sum = sums[at];
-        float *out = a.out + (size_t)(row0 + rr / a.group) * a.out_stride + (size_t)(kvh * a.group + rr % a.group) * hd + d;
-        out[0] = sum == 0.0f ? 0.0f : y0 / sum;
-        out[1] = sum == 0.0f ? 0.0f : y1 / sum;
+        wait_fetches<0>();
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < some * pairs; i += 256u) {
+            const uint32_t at = r0 + i / pairs, d = 2u * (i % pairs);
+            float y0 = 0.0f, y1 = 0.0f;
+            for (uint32_t s = 0; s < parts; ++s) {
+                const float *u = (const float *)(lds + s * pieces * 1024u) + 2u * i;
+                const float f = factor[s][at];
+                y0 += f != 0.0f ? f * u[0] : 0.0f;
+                y1 += f != 0.0f ? f * u[1] : 0.0f;
+            }
+            const uint32_t rr = tile * 128u + at;
+            float *out = a.out + (size_t)(row0 + rr / a.group) * a.out_stride + (size_t)(kvh * a.group + rr % a.group) * hd + d;
+            out[0] = y0;
+            out[1] = y1;
+        }
     }
 }
 

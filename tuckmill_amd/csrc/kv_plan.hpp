@@ -55,14 +55,19 @@ inline AttnPlan decode_plan(uint32_t type_id, uint32_t seqs, uint32_t q_heads, u
 
 constexpr uint32_t PREFILL_ROWS = 128; // query rows x heads of a workgroup
 constexpr uint32_t PREFILL_MAX_SPLITS = 8;
+// Where tiles leave CUs without one their positions are shared, eight steps of 64 at least (in us,
+// with 2, 4 and 8: 512 rows of 128 channels on 64 cached 43, 42, 30, on 16000 154 each).
+constexpr uint32_t PREFILL_MIN_STEPS = 8;
+constexpr uint32_t PREFILL_SHARES = 256; // (512: 256 rows on 16000 cached 118 for 92)
 constexpr uint64_t PREFILL_MAX_GROUPS = 1u << 23;
-// Up to this many units the decode kernel takes ragged rows. (In us, it and the prefill
-// kernel: at 512 units of 128 channels 25 and 55, at 1024 54 and 67 or 83 and 81, at
-// 2048 135 and 102; of 64 channels at 1024 50 and 60, at 2048 62 and 77; of 256 channels at
-// 2000 137 and 200, at 4000 500 and 357.) Pages of f32 it takes always: their products go at
+// Up to this many units the decode kernel takes ragged rows. (In us, it and the prefill kernel, on up
+// to 64, 2000 and 16000 cached positions: of 128 channels at 1032 units 20, 39, 127 and 21, 53, 92, at
+// 2056 38, 66, 281 and 30, 57, 153; of 64 channels at 776 11, 15, 33 and 14, 22, 36, at 1544 21, 35, 88
+// and 20, 32, 58; of 256 channels at 516 26, 43, 152 and 52, 105, 190, at 1028 58, 92, 490 and 91, 120,
+// 333.) Pages of f32 it takes always: their products go at
 // a sixteenth of f16's rate, and its waves of 16 rows fill the card better than tiles of
 // 128 did (1500 rows of 256 channels 69 and 138, 4000 926 and 1216, 4000 of 128 347 and 509).
-constexpr uint64_t DECODE_MAX_UNITS = 1024;
+constexpr uint64_t DECODE_MAX_UNITS = 1056;
 
 // Ragged rows. How they fall to sequences is known on the device only: every
 // sequence may have one tile that is not full. Where that leaves few workgroups the
@@ -84,8 +89,8 @@ inline AttnPlan prefill_plan(uint32_t type_id, uint32_t seqs, uint32_t tokens, u
     p.tiled = true;
     p.tile_bound = tiles_of(PREFILL_ROWS);
     const uint64_t units = p.tile_bound * kv_heads;
-    uint64_t splits = units < 256u ? (512u + units - 1u) / units : 1u;
-    const uint64_t most = (positions + 255u) / 256u;
+    uint64_t splits = units < PREFILL_SHARES ? (PREFILL_SHARES + units - 1u) / units : 1u;
+    const uint64_t most = positions / (64u * PREFILL_MIN_STEPS);
     splits = splits < most ? splits : most;
     p.splits = (uint32_t)(splits < 1u ? 1u : splits > PREFILL_MAX_SPLITS ? PREFILL_MAX_SPLITS : splits);
     if (p.splits > 1u) {

@@ -85,7 +85,6 @@ template <bool RAGGED> hipError_t launch_decode(hipStream_t stream, hipEvent_t s
 
 template <int D, int W> hipError_t launch_prefill_as(hipStream_t stream, hipEvent_t stop, const kv::PrefillArgs &args) {
     constexpr uint32_t LDS = 4u * kv::PrefillShape<D>::BYTES;
-    static_assert(LDS >= 128u * (kv::PREFILL_MAX_SPLITS + 1u) * 4u, "factors and sums of a join");
     const dim3 grid(args.a.cache.kv_heads * args.splits * args.tile_bound);
     return args.a.cache.head_dim == (uint32_t)D
                ? launch_lds<LDS, kv::attn_prefill_kernel<D, true, W>>(stream, stop, grid, dim3(256), args)
