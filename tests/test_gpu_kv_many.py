@@ -262,3 +262,32 @@ def test_logits_with_long_lists(ctx, rows, vocab, hist, biases):
     ctx.fence()
     want, tol = K.adjust(x, history, hl, pen, ids, values, bl)
     K.near(f32(out, x.shape), want, tol)
+
+
+@pytest.mark.parametrize("type_id,heads,kv_heads", [(K.F16, 4, 2), (K.F32, 4, 2), (K.F16, 64, 64)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_infinite_queries_keep_to_themselves(ctx, type_id, heads, kv_heads, d):
+    rng = np.random.default_rng(41)
+    news, lens = [130, 6], [150, 40]
+    paged = K.Paged(rng, type_id, 16, kv_heads, d, lens)
+    for s in range(2):
+        paged.keys[s][:, :, 5] = -np.abs(paged.keys[s][:, :, 5]) - 1
+        for j in range(lens[s]):
+            paged.put(s, j)
+    starts, _, _ = prefill_case(rng, news, lens)
+    q = rng.standard_normal((136, heads, d)).astype(np.float32)
+    q[17] = 0
+    q[17, :, 5] = np.inf  # every score is -infinity
+    q[40, :, 5] = -np.inf  # every score is infinity
+    q[41] *= 1e30
+    q[42] *= 1e-30
+    with np.errstate(all="ignore"):
+        want, tol = want_prefill(paged, q.reshape(136, -1), heads, starts, news, 0.01)
+        got = run_prefill(ctx, paged, q.reshape(136, -1), heads, H.Attention(0.01), starts)
+    rest = np.ones(136, bool)
+    rest[[17, 40, 41]] = False
+    K.near(got[rest], want[rest], tol[rest])
+    assert not got[17].any() or np.isnan(got[17]).all()  # (zero times infinity is NaN, as in a plain product)
+    assert np.isnan(got[40]).all()
+    near_one = np.abs(got[41]) <= np.abs(paged.values[0]).max() * (1 + 2.0 ** -20)  # (one weight is all, whichever)
+    assert near_one.all()

@@ -57,14 +57,23 @@ template <int D, bool FULL> struct Tile<_Float16, D, FULL> {
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
         const int by = scale_bits(top);
+        const float scale = ldexpf(sign, by);
+        float minus = -1.0f; // (for one instruction that takes the f16 where it is)
+        asm("" : "+s"(minus));
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float y = ldexpf(x[s][j] * sign, by);
-                const _Float16 hi = (_Float16)y;
-                const float rest = fabsf((float)hi) < INFINITY ? y - (float)hi : 0.0f;
-                q[s][j] = c < 8u ? hi : (_Float16)rest;
+                const float y = x[s][j] * scale;
+                const float rest = fmaf((float)(_Float16)y, minus, y);
+                q[s][j] = (_Float16)(c < 8u ? y : rest);
+            }
+        }
+        if (__any(!(top < INFINITY))) {
+            const bool none = c >= 8u && !(top < INFINITY);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                q[s] = none ? Unit{} : q[s];
             }
         }
         return ldexpf(1.0f, -by);

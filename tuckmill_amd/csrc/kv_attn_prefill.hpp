@@ -37,16 +37,16 @@ template <int D, bool FULL> struct Rows {
     typedef f16x8 Unit;
     Unit hi[S::KS], lo[S::KS]; // q in two parts (22 bits of the row's largest magnitude)
 
-    __device__ __forceinline__ float load_q(const float *row, uint32_t h, uint32_t hd, bool live) {
+    // (a lane without a row is given one that is there: its results are not used)
+    __device__ __forceinline__ float load_q(const float *row, uint32_t h, uint32_t hd, float minus) {
         float top = 0.0f;
         auto read = [&](float (&x)[8], int s) {
             const uint32_t d = 8u * (2u * s + h);
-            const bool there = live && (FULL || d < hd);
             const float *from = row + (FULL || d < hd ? d : 0u);
             const f32x4 y[2] = {*(const f32x4_unaligned *)from, *(const f32x4_unaligned *)(from + 4)};
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                x[j] = there ? y[j / 4][j % 4] : 0.0f;
+                x[j] = FULL || d < hd ? y[j / 4][j % 4] : 0.0f;
             }
         };
 #pragma unroll
@@ -60,16 +60,23 @@ template <int D, bool FULL> struct Rows {
         }
         top = fmaxf(top, __shfl_xor(top, 32));
         const int by = scale_bits(top);
+        const float scale = ldexpf(1.0f, by);
+        const bool finite = top < INFINITY; // (what is not goes whole into the first part)
 #pragma unroll
         for (int s = 0; s < S::KS; ++s) {
             float x[8];
             read(x, s);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float y = ldexpf(x[j], by);
-                hi[s][j] = (_Float16)y;
-                const float whole = (float)hi[s][j];
-                lo[s][j] = (_Float16)(fabsf(whole) < INFINITY ? y - whole : 0.0f);
+            for (int j = 0; j < 8; j += 2) {
+                const f32x2 y = {x[j] * scale, x[j + 1] * scale};
+                const f16x2 first = __builtin_convertvector(y, f16x2);
+                const f32x2 rest = {finite ? fmaf((float)first[0], minus, y[0]) : 0.0f,
+                                    finite ? fmaf((float)first[1], minus, y[1]) : 0.0f};
+                const f16x2 second = __builtin_convertvector(rest, f16x2);
+                hi[s][j] = first[0];
+                hi[s][j + 1] = first[1];
+                lo[s][j] = second[0];
+                lo[s][j + 1] = second[1];
             }
         }
         return ldexpf(1.0f, -by);
@@ -230,8 +237,10 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
         look_up(s_begin);
         fetch(s_begin, 0u);
     }
+    float minus = -1.0f;
+    asm("" : "+s"(minus));
     R q;
-    const float unscale = q.load_q(a.q + (size_t)row * a.q_stride + (size_t)head * hd, h, hd, live);
+    const float unscale = q.load_q(a.q + (size_t)row * a.q_stride + (size_t)head * hd, h, hd, minus);
     const float slope = a.slopes != nullptr ? a.slopes[head] * LOG2E : 0.0f;
     const float to_log2 = score_factor(a.scale * unscale, a.softcap);
     const float cap_log2 = a.softcap * LOG2E;
@@ -375,8 +384,6 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
                 l += x[b][v];
             }
         }
-        float minus = -1.0f;
-        asm("" : "+s"(minus));
         auto v_of = [&](int t, int i) { return (v_row ^ (32u * i)) + t * (32u * 128u); };
         if (!whole) {
             // A value that is not finite must not reach a row that does not see it through
