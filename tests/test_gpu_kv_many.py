@@ -291,3 +291,25 @@ def test_infinite_queries_keep_to_themselves(ctx, type_id, heads, kv_heads, d):
     assert np.isnan(got[40]).all()
     near_one = np.abs(got[41]) <= np.abs(paged.values[0]).max() * (1 + 2.0 ** -20)  # (one weight is all, whichever)
     assert near_one.all()
+
+
+@pytest.mark.parametrize("type_id,kv_heads,news", [(K.F16, 32, 200), (K.F16, 2, 5), (K.F32, 2, 5)])
+def test_nan_that_is_seen_shows_where_its_weight_is_nothing(ctx, type_id, kv_heads, news):
+    """Among positions shared between workgroups, in a part whose scores are far below the rest."""
+    rng = np.random.default_rng(42)
+    paged = K.Paged(rng, type_id, 64, kv_heads, 64, [3000])
+    paged.keys[0][:1000, :, 0] = -3000
+    paged.keys[0][1000:, :, 0] = 0
+    paged.values[0][10, :, 3] = np.nan
+    for j in range(3000):
+        paged.put(0, j)
+    q = rng.standard_normal((news, kv_heads, 64)).astype(np.float32)
+    q[:, :, 0] = 5
+    got = run_prefill(ctx, paged, q.reshape(news, -1), kv_heads, H.Attention(0.125), np.array([0, news]))
+    assert np.isnan(got[..., 3]).all()
+    paged.values[0][10, :, 3] = 0  # (in the reference; the cache holds it still)
+    want, tol = want_prefill(paged, q.reshape(news, -1), kv_heads, np.array([0, news]), [news], 0.125)
+    K.near(np.delete(got, 3, -1), np.delete(want, 3, -1), np.delete(tol, 3, -1))
+    if news == 5:
+        got = run_decode(ctx, paged, q[0].reshape(1, -1), kv_heads, H.Attention(0.125))
+        assert np.isnan(got[..., 3]).all() and np.isfinite(np.delete(got, 3, -1)).all()

@@ -576,8 +576,8 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
             for (uint32_t s = 0; s < parts; ++s) {
                 const float *u = (const float *)(lds + s * pieces * 1024u) + 2u * i;
                 const float f = factor[s][at];
-                y0 += f != 0.0f ? f * u[0] : 0.0f;
-                y1 += f != 0.0f ? f * u[1] : 0.0f;
+                y0 += f * u[0];
+                y1 += f * u[1];
             }
             const uint32_t rr = tile * 128u + at;
             float *out = a.out + (size_t)(row0 + rr / a.group) * a.out_stride + (size_t)(kvh * a.group + rr % a.group) * hd + d;

@@ -31,7 +31,7 @@ template <> __device__ __forceinline__ float to_page<float>(float x) { return x;
 template <> __device__ __forceinline__ _Float16 to_page<_Float16>(float x) { return (_Float16)x; }
 
 constexpr uint32_t ROPE_ROWS = 16;    // rows of a workgroup
-constexpr uint32_t ROPE_HEADS = 8;    // heads of q and k it turns
+constexpr uint32_t ROPE_HEADS = 16;   // heads of q and k it turns (4, 8, 16: 49.3, 48.5, 47.0 us below)
 constexpr uint32_t ROPE_CHANNELS = 256; // channels of v it stores
 
 // Four f32 as the page's type, in one piece.
@@ -41,12 +41,12 @@ __device__ __forceinline__ void store4(_Float16 *at, f32x4 x) {
     *(f16x4 *)at = f16x4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
 }
 
-// Workgroups of 16 rows: blockIdx.y names eight heads of q and k, or behind those 256
+// Workgroups of 16 rows: blockIdx.y names sixteen heads of q and k, or behind those 256
 // channels of v. The angles of the rows are taken once per workgroup, into LDS; heads
 // go four pairs a thread (WIDE: everything is aligned for 16-byte pieces). v is
 // stored with a channel's places side by side, so there the lanes of a wave are rows:
 // rows that follow each other in the cache make up a line between them. Bound by the
-// stream of q, k and v.
+// stream of q, k and v: 4093 rows of 32 and 8 heads of 128 channels, 184 MB, 47 us = 3.9 TB/s.
 template <typename T, bool WIDE> __global__ __launch_bounds__(256) void rope_store_kernel(RopeArgs a) {
     constexpr int W = WIDE ? 4 : 1;
     __shared__ float angle[2][ROPE_ROWS][128];
