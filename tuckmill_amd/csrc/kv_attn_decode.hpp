@@ -321,11 +321,8 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, 2) void attn_decode_kernel(Decod
         uint64_t before = 0, upto = 0; // `before`: of the sequences before s0
         auto add_up = [&]() {
             const uint64_t shares = size != 0u ? (steps_here + size - 1u) / size : 0u;
-            upto = (uint64_t)units_of(rows_here) * (size == 0u ? steps_here : shares > 1u ? shares | shares << 32 : shares);
-            for (uint32_t x = 1; x <= last_lane(a); x <<= 1) {
-                const uint64_t y = __shfl_up(upto, x);
-                upto += lane >= x ? y : 0u;
-            }
+            upto = sum_over_lanes((uint64_t)units_of(rows_here) *
+                                  (size == 0u ? steps_here : shares > 1u ? shares | shares << 32 : shares));
         };
         auto look = [&]() {
             rows_up_to = highest;
@@ -337,7 +334,7 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, 2) void attn_decode_kernel(Decod
             add_up();
         };
         auto look_on = [&]() {
-            before += __shfl(upto, last_lane(a));
+            before += last_of(upto);
             highest = rows_up_to;
             s0 += 64u;
             look();
@@ -346,7 +343,7 @@ __global__ __launch_bounds__(64 * DECODE_WAVES, 2) void attn_decode_kernel(Decod
         while (s0 + 64u < a.seqs) {
             look_on();
         }
-        size = (uint32_t)((before + __shfl(upto, last_lane(a)) + args.shares - 1u) / args.shares);
+        size = (uint32_t)((before + last_of(upto) + args.shares - 1u) / args.shares);
         size = __builtin_amdgcn_readfirstlane(max(size, 1u));
         before = 0;
         if (s0 == 0u) {

@@ -158,9 +158,28 @@ __device__ __forceinline__ int most64(int x) {
                max(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48)));
 }
 
-// The last lane of a wave that goes through the sequences, one a lane: sums and maxima over the lanes
-// before each stop there (a few sequences need few steps).
-__device__ __forceinline__ uint32_t last_lane(const AttnArgs &a) { return min(a.seqs, 64u) - 1u; }
+// Sums and maxima over the lanes up to each, within rows of 16 and then from row to row.
+template <int CONTROL, int ROWS> __device__ __forceinline__ uint32_t moved(uint32_t x) { // 0 where nothing comes from
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CONTROL, ROWS, 0xf, false);
+}
+template <int CONTROL, int ROWS> __device__ __forceinline__ uint64_t moved(uint64_t x) {
+    return (uint64_t)moved<CONTROL, ROWS>((uint32_t)(x >> 32)) << 32 | moved<CONTROL, ROWS>((uint32_t)x);
+}
+template <typename U, typename OP> __device__ __forceinline__ U over_lanes(U x, OP op) {
+    x = op(x, moved<0x111, 0xf>(x)); // from 1, 2, 4 and 8 lanes before
+    x = op(x, moved<0x112, 0xf>(x));
+    x = op(x, moved<0x114, 0xf>(x));
+    x = op(x, moved<0x118, 0xf>(x));
+    x = op(x, moved<0x142, 0xa>(x)); // from the end of the row before, to the second and fourth
+    return op(x, moved<0x143, 0xc>(x)); // from the end of the second, to the third and fourth
+}
+template <typename U> __device__ __forceinline__ U sum_over_lanes(U x) {
+    return over_lanes(x, [](U a, U b) { return a + b; });
+}
+__device__ __forceinline__ uint32_t last_of(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); }
+__device__ __forceinline__ uint64_t last_of(uint64_t x) {
+    return (uint64_t)last_of((uint32_t)(x >> 32)) << 32 | last_of((uint32_t)x);
+}
 
 // Rows of sequence s0 + lane of a ragged batch, for a wave that goes through the sequences 64
 // at a time, and the first of them (`highest`: of the bounds before). A sequence has rows where its bounds ascend
@@ -169,13 +188,9 @@ __device__ __forceinline__ uint32_t last_lane(const AttnArgs &a) { return min(a.
 __device__ __forceinline__ uint32_t rows_of(const AttnArgs &a, uint32_t s0, uint32_t &highest, uint32_t &first) {
     const uint32_t lane = threadIdx.x & 63u, s = min(s0 + lane, a.seqs - 1u);
     const uint32_t r0 = a.starts[s], r1 = a.starts[s + 1u];
-    uint32_t above = first = r0;
-    for (uint32_t x = 1; x <= last_lane(a); x <<= 1) {
-        const uint32_t y = __shfl_up(above, x);
-        above = lane >= x ? max(above, y) : above;
-    }
-    above = max(above, highest);
-    highest = __shfl(above, last_lane(a));
+    first = r0;
+    const uint32_t above = max(over_lanes(r0, [](uint32_t x, uint32_t y) { return max(x, y); }), highest);
+    highest = last_of(above);
     return s0 + lane < a.seqs && r0 == above && r0 <= r1 && r1 <= a.tokens ? r1 - r0 : 0u;
 }
 
@@ -196,11 +211,7 @@ __device__ __forceinline__ uint32_t find_tile(const AttnArgs &a, uint32_t tile_r
             if (pass == 0 || a.seqs > 64u) {
                 n = rows_of(a, s0, highest, first) * a.group;
                 mine = (n + tile_rows - 1u) / tile_rows;
-                upto = mine;
-                for (uint32_t x = 1; x <= last_lane(a); x <<= 1) {
-                    const uint32_t y = __shfl_up(upto, x);
-                    upto += lane >= x ? y : 0u;
-                }
+                upto = sum_over_lanes(mine);
             }
             if (pass == 1) {
                 const uint64_t found = __ballot(want < before + upto);
@@ -213,7 +224,7 @@ __device__ __forceinline__ uint32_t find_tile(const AttnArgs &a, uint32_t tile_r
                     here = true;
                 }
             }
-            before += __shfl(upto, last_lane(a));
+            before += last_of(upto);
         }
         if (pass == 0) {
             if (index >= before) {
