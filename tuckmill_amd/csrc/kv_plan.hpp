@@ -100,7 +100,8 @@ inline AttnPlan prefill_plan(uint32_t type_id, uint32_t seqs, uint32_t tokens, u
     return p;
 }
 
-// Ids of a workgroup that adjusts logits: large tiles where they still give every CU one.
+// Ids of a workgroup that adjusts logits: large tiles where they still give every CU one. (In us, large
+// and small, rows of 151936: one 7.9 and 6.1, 16 8.0 and 6.2, 64 with histories of 4096 20 and 30.)
 constexpr uint32_t LOGITS_LARGE = 8192, LOGITS_SMALL = 1024, LOGITS_MIN_GROUPS = 256;
 
 } // namespace kv
