@@ -401,7 +401,8 @@ int tm_hip_attn_decode_f32(tm_hip_ctx *ctx, const tm_hip_attn *attn, const tm_hi
  * them). Rows in no sequence keep what out held: those behind starts[seqs], and
  * those of a sequence whose two bounds do not ascend within `tokens`, or whose
  * first is below an earlier entry. Otherwise as tm_hip_attn_decode_f32;
- * attn->first has an entry per row. */
+ * attn->first has an entry per row. (Of f32 pages, more than 2^23 tiles of sixteen rows
+ * over all key-value heads are refused; of F16 pages, of 128 rows.) */
 int tm_hip_attn_prefill_f32(tm_hip_ctx *ctx, const tm_hip_attn *attn, const tm_hip_kv_cache *cache,
                             tm_hip_buffer *q, tm_hip_buffer *table, tm_hip_buffer *lens,
                             tm_hip_buffer *starts, tm_hip_buffer *out, uint32_t tokens,

@@ -270,3 +270,66 @@ def test_refused_calls_leave_an_open_group_as_it_was(call, ctx):
     ctx.end_group()
     ctx.fence()
     assert np.isfinite(ctx.last_gpu_ms())
+
+
+PLAN = r"""
+#include "kv_plan.hpp"
+#include <cstdio>
+#include <random>
+#include <vector>
+#define CHECK(x) do { if (!(x)) { printf("line %d: %s\n", __LINE__, #x); return 1; } } while (0)
+int main() {
+    std::mt19937_64 r(5);
+    auto up_to = [&](uint64_t n) { return r() % n + 1u; };
+    for (int i = 0; i < 200000; ++i) {
+        const uint32_t type = r() % 2u, kv = 1u << r() % 8u, group = up_to(16), d = 8u * up_to(32), cols = kv::decode_cols(type);
+        const uint32_t seqs = up_to(r() % 2u ? 8u : 600u), tokens = up_to(r() % 2u ? 64u : 20000u);
+        const uint64_t positions = 16u * up_to(r() % 2u ? 16u : 1u << 20);
+        const kv::AttnPlan p = i % 2 ? kv::prefill_plan(type, seqs, tokens, kv * group, kv, d, positions)
+                                     : kv::decode_plan(type, seqs, kv * group, kv, d, positions);
+        if (p.tiled) { // every tile and part has a slot of its own
+            CHECK(type == 1u && p.splits >= 1u && p.splits <= kv::PREFILL_MAX_SPLITS);
+            CHECK(p.tile_bound >= ((uint64_t)tokens * group + 127u) / 128u && p.tile_bound <= (uint64_t)tokens * group);
+            CHECK(p.splits == 1u || (p.arrivals == p.tile_bound * kv && p.partial_floats == p.arrivals * p.splits * 128u * (d + 2u)));
+            continue;
+        }
+        if (p.shares == 0u) {
+            CHECK(i % 2 == 0 && seqs > kv::DECODE_MAX_SEQS);
+            continue;
+        }
+        // sequences of any rows and steps, as the kernel deals them out
+        std::vector<uint64_t> units, steps;
+        uint64_t total = 0, left = tokens;
+        for (uint32_t s = 0; s < seqs; ++s) {
+            const uint64_t rows = i % 2 ? std::min<uint64_t>(left, r() % (2u * tokens / seqs + 2u)) : 1u;
+            left -= i % 2 ? rows : 0u;
+            units.push_back(i % 2 ? (rows * group + cols - 1u) / cols * kv : (group + cols - 1u) / cols * kv);
+            const uint64_t n = r() % 3u ? r() % 5u * r() % (positions + 1u) : positions, tile = 4u * (type ? 32u : 16u);
+            steps.push_back(std::max<uint64_t>(1u, (std::min(n, positions) + tile - 1u) / tile));
+            total += units.back() * steps.back();
+        }
+        const uint64_t size = std::max<uint64_t>(1u, (total + p.shares - 1u) / p.shares);
+        uint64_t groups = 0, slots = 0;
+        for (uint32_t s = 0; s < seqs; ++s) {
+            const uint64_t parts = (steps[s] + size - 1u) / size;
+            groups += units[s] * parts;
+            slots += parts > 1u ? units[s] * parts : 0u;
+        }
+        CHECK(groups <= p.grid);
+        CHECK(slots <= p.arrivals && p.partial_floats == p.arrivals * cols * (d + 2u));
+    }
+    return 0;
+}
+"""
+
+
+def test_shares_fit_the_launch_and_the_workspace(tmp_path):
+    """Any sequences a call may hold: as many workgroups as are launched have their shares, and parts
+    that others have a part beside have a slot."""
+    src, out = tmp_path / "plan.cpp", tmp_path / "plan"
+    src.write_text(PLAN)
+    gxx = shutil.which(os.environ.get("CXX", "g++"))
+    res = subprocess.run([gxx, "-std=c++17", "-O2", "-I", CSRC, "-o", str(out), str(src)], capture_output=True, text=True)
+    assert res.returncode == 0, res.stderr
+    res = subprocess.run([str(out)], capture_output=True, text=True, timeout=120)
+    assert res.returncode == 0, res.stdout
