@@ -562,7 +562,7 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
         }
 #pragma unroll
         for (uint32_t s = 0; s < PREFILL_MAX_SPLITS; ++s) {
-            factor[s][threadIdx.x] = sum == 0.0f ? 0.0f : t[s] / sum;
+            factor[s][threadIdx.x] = sum == 0.0f ? -1.0f : t[s] / sum; // (-1: the row's result is zero)
         }
     }
     const uint32_t row_bytes = hd * 4u;
@@ -587,8 +587,9 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
             }
             const uint32_t rr = tile * 128u + at;
             float *out = a.out + (size_t)(row0 + rr / a.group) * a.out_stride + (size_t)(kvh * a.group + rr % a.group) * hd + d;
-            out[0] = y0;
-            out[1] = y1;
+            const bool none = factor[0][at] < 0.0f; // (whatever the values: a part of no weight may hold NaN)
+            out[0] = none ? 0.0f : y0;
+            out[1] = none ? 0.0f : y1;
         }
     }
 }
