@@ -408,20 +408,35 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
                 any = any || bad[j] != (T)0.0f;
             }
             if (__any(any)) {
-                if (lane == 0u) {
-                    cleaned = 1u;
+                // (only what some row of the workgroup sees is worth telling: places behind the
+                // sequence or in a page that is not there hold anything)
+                const int seen_lo = min(min(range[0][0], range[1][0]), min(range[2][0], range[3][0])) - mine;
+                const int seen_hi = max(max(range[0][1], range[1][1]), max(range[2][1], range[3][1])) - mine;
+                uint32_t there = 0;
+#pragma unroll
+                for (int i = 0; i < PAGES; ++i) {
+                    there |= pages[i] < a.cache.pages ? 1u << i : 0u;
                 }
+                uint32_t tell = 0;
 #pragma unroll 1
                 for (int t = 0; t < S::DT; ++t) {
 #pragma unroll 1
                     for (int i = 0; i < R::PIECES; ++i) {
                         Unit v = *(Lds)v_of(t, i);
+                        uint32_t wrong = 0;
 #pragma unroll
                         for (int j = 0; j < S::E; ++j) {
-                            v[j] = fabsf((float)v[j]) < INFINITY ? v[j] : (T)0.0f;
+                            const bool finite = fabsf((float)v[j]) < INFINITY;
+                            wrong |= finite ? 0u : 1u << j;
+                            v[j] = finite ? v[j] : (T)0.0f;
                         }
                         *(__attribute__((address_space(3))) Unit *)v_of(t, i) = v;
+                        const int first = min(max(seen_lo - 16 * i, 0), S::E), last = min(max(seen_hi - 16 * i, first), S::E);
+                        tell |= (there >> i & 1u) != 0u ? wrong & ((1u << last) - (1u << first)) : 0u;
                     }
+                }
+                if (__any(tell != 0u) && lane == 0u) {
+                    cleaned = 1u;
                 }
             }
         }
