@@ -1,4 +1,6 @@
-"""Paged attention at its edges."""
+"""Paged attention at its edges: scores of minus infinity, scores that overflow, unused places of a cache
+that hold anything. Comparisons ask first that their tolerances are numbers: an infinite or undefined
+one would accept any result."""
 import numpy as np
 import pytest
 
@@ -6,7 +8,7 @@ import kvutil as K
 from tuckmill_amd import hip as H
 
 from q8util import require_gpu, upload_new
-from test_gpu_kv import f32, run_decode, run_prefill
+from test_gpu_kv import f32, run_decode, run_prefill, want_decode
 from test_gpu_kv_many import many
 
 pytestmark = pytest.mark.gpu
@@ -17,6 +19,86 @@ def ctx():
     c = require_gpu()
     yield c
     c.close()
+
+
+def near(got, want, tol, what=""):
+    assert np.isfinite(np.broadcast_to(tol, np.shape(want))[np.isfinite(want)]).all(), f"{what}: tolerances"
+    K.near(got, want, tol, what)
+
+
+def test_a_tolerance_that_is_no_number_is_refused():
+    with pytest.raises(AssertionError, match="tolerances"):
+        near(np.array([1e9]), np.array([0.5]), np.array([np.nan]))
+
+
+# ---- a score of minus infinity takes its own position out, and no other ---------------------------
+
+@pytest.mark.parametrize("type_id", [K.F16, K.F32])
+@pytest.mark.parametrize("d", [64, 128, 256, 72])
+def test_decode_one_infinite_score_takes_its_position_out(ctx, type_id, d):
+    """A key with a channel of -infinity under positive queries: the softmax gives it a weight of
+    exactly zero, so what is left is the attention over the other positions."""
+    rng = np.random.default_rng(50 + d)
+    lens, heads = [100, 33, 1, 700], 3
+    out_of = [50, 0, 0, 699]
+    paged = K.Paged(rng, type_id, 32, 1, d, lens)
+    seen = [np.ones(n, bool) for n in lens]
+    for s, j in enumerate(out_of):
+        paged.keys[s][j, 0, 3] = -np.inf
+        paged.put(s, j)
+        seen[s][j] = False
+    q = np.abs(rng.standard_normal((len(lens), heads * d))).astype(np.float32) + np.float32(0.1)
+    got = run_decode(ctx, paged, q, heads, H.Attention(0.125))
+    clean = K.Paged(rng, type_id, 32, 1, d, lens)
+    clean.keys = [np.where(np.isinf(k), 0, k) for k in paged.keys]  # (where it is not looked at)
+    clean.values = paged.values
+    want, tol = want_decode(clean, q, heads, 0.125, seen=seen)
+    near(got, want, tol)
+    assert not got[2].any()  # the only position it had
+
+
+# ---- huge queries --------------------------------------------------------------------------------
+
+def check_decided(got, scores, error, values, margin):
+    """got [channel] where the largest of `scores` (each off by at most `error`) decides alone: the
+    value at that position if no other's score comes within the two errors and `margin`, else
+    something between the values."""
+    order = np.argsort(scores)
+    top, second = order[-1], order[-2]
+    if scores[top] - scores[second] > error[top] + error[second] + margin:
+        # (one weight, in two parts of 22 bits, and nothing beside it: half steps 2 for the parts, 1 for the
+        # products, 2 for the sum of weights, 2 for the join, 1 for the division)
+        assert np.abs(got - values[top]).max() <= 8 * K.EPS * np.abs(values[top]).max()
+        return 1
+    assert (got >= values.min(0) - 1e-5).all() and (got <= values.max(0) + 1e-5).all()
+    return 0
+
+
+@pytest.mark.parametrize("type_id,heads,rows", [(K.F16, 2, 1), (K.F32, 2, 1), (K.F16, 2, 6), (K.F32, 2, 6), (K.F16, 64, 140)])
+@pytest.mark.parametrize("size", [1e10, 1e30])
+def test_huge_queries_take_the_value_of_the_largest_score(ctx, type_id, heads, rows, size):
+    rng = np.random.default_rng(60)
+    d, n = 64, 300
+    paged = K.Paged(rng, type_id, 16, heads, d, [n])
+    q = (rng.standard_normal((rows, heads * d)) * size).astype(np.float32)
+    attn = H.Attention(d ** -0.5)
+    if rows == 1:
+        got = run_decode(ctx, paged, q, heads, attn)
+    else:
+        assert many(rows, 1, heads, heads) == (rows > 100)
+        got = run_prefill(ctx, paged, q, heads, attn, np.array([0, rows]))
+    decided = 0
+    for r in range(rows):
+        upto = n - rows + r + 1
+        for h in range(heads):
+            k = paged.keys[0][:upto, h].astype(np.float64)
+            qh = q[r].reshape(heads, d)[h].astype(np.float64)
+            x = d ** -0.5 * (k @ qh)
+            # f32 sums of d products, and q in 22 bits of its largest magnitude
+            e = d ** -0.5 * (np.abs(k) @ np.abs(qh) * K.SIGMAS * np.sqrt(d) * K.EPS +
+                             np.abs(k).sum(1) * np.abs(qh).max() * 2.0 ** -22) + 8 * K.EPS * np.abs(x)
+            decided += check_decided(got[r, h], x, e, paged.values[0][:upto, h].astype(np.float64), 200.0)
+    assert decided >= 0.9 * rows * heads  # (the check is not an empty one)
 
 
 @pytest.mark.parametrize("rows,heads", [(1, 2), (6, 2), (200, 64)])
