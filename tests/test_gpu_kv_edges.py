@@ -1,6 +1,10 @@
 """Paged attention at its edges: scores of minus infinity, scores that overflow, unused places of a cache
-that hold anything. Comparisons ask first that their tolerances are numbers: an infinite or undefined
+that hold anything, first launches inside a recorded step. Comparisons ask first that their tolerances are numbers: an infinite or undefined
 one would accept any result."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -12,6 +16,7 @@ from test_gpu_kv import f32, run_decode, run_prefill, want_decode
 from test_gpu_kv_many import many
 
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 @pytest.fixture(scope="module")
@@ -154,3 +159,63 @@ def test_what_lies_behind_a_sequence_costs_nothing(ctx):
             got[i] = f32(out, (sum(news), heads * d)).view(np.uint32)
     assert np.array_equal(got[0], got[1])
     assert min(times[0]) <= 1.5 * min(times[1]), (min(times[0]), min(times[1]))
+
+
+# ---- recorded steps -------------------------------------------------------------------------------
+
+def test_first_launches_inside_a_recorded_step():
+    """In a process of its own, so that nothing has launched these kernels before: the forms whose LDS has
+    to be allowed first, recorded, replayed, and run again without a recording."""
+    code = """
+import sys
+sys.path.insert(0, "tests")
+import numpy as np
+import kvutil as K
+from tuckmill_amd import hip as H
+from q8util import upload_new
+from test_gpu_kv import f32, want_decode, want_prefill
+ctx = H.HipContext.open()
+rng = np.random.default_rng(80)
+for type_id, heads, kv_heads, d, lens in ((K.F16, 16, 8, 128, [700, 65]), (K.F32, 4, 2, 128, [300, 9]), (K.F16, 4, 1, 256, [500, 40]),
+                                          (K.F32, 4, 1, 256, [200, 31])):
+    paged = K.Paged(rng, type_id, 64, kv_heads, d, lens)
+    q = rng.standard_normal((2, heads * d)).astype(np.float32)
+    out, cache, attn = ctx.buffer(q.nbytes), paged.upload(ctx), H.Attention(d ** -0.5)
+    bufs = [upload_new(ctx, x) for x in (q, paged.table, K.u32(lens))]
+    ctx.begin_group()
+    ctx.attn_decode(attn, cache, *bufs, out, 2, heads, paged.stride)
+    step = ctx.end_group_recorded()
+    want, tol = want_decode(paged, q, heads, float(np.float32(d ** -0.5)))
+    for turn in range(3):
+        out.zero(0, out.len())
+        step.run()
+        ctx.fence()
+        got = f32(out, want.shape)
+        K.near(got, want, tol, f"decode {type_id} {d} {turn}")
+    ctx.attn_decode(attn, cache, *bufs, out, 2, heads, paged.stride)
+    ctx.fence()
+    assert np.array_equal(f32(out, want.shape).view(np.uint32), got.view(np.uint32))
+for type_id, heads, d, news, lens in ((K.F16, 64, 128, [100, 60], [150, 60]), (K.F16, 64, 256, [100, 60], [150, 60]),
+                                      (K.F16, 4, 128, [5, 3], [150, 60]), (K.F32, 4, 256, [5, 30], [150, 60])):
+    paged = K.Paged(rng, type_id, 64, heads, d, lens)
+    starts = np.concatenate([[0], np.cumsum(news)])
+    q = rng.standard_normal((int(starts[-1]), heads * d)).astype(np.float32)
+    out, cache, attn = ctx.buffer(q.nbytes), paged.upload(ctx), H.Attention(d ** -0.5)
+    bufs = [upload_new(ctx, x) for x in (q, paged.table, K.u32(lens), K.u32(starts))]
+    ctx.begin_group()
+    ctx.attn_prefill(attn, cache, *bufs, out, len(q), 2, heads, paged.stride)
+    step = ctx.end_group_recorded()
+    want, tol = want_prefill(paged, q, heads, starts, news, float(np.float32(d ** -0.5)))
+    for turn in range(3):
+        out.zero(0, out.len())
+        step.run()
+        ctx.fence()
+        got = f32(out, want.shape)
+        K.near(got, want, tol, f"prefill {type_id} {d} {turn}")
+    ctx.attn_prefill(attn, cache, *bufs, out, len(q), 2, heads, paged.stride)
+    ctx.fence()
+    assert np.array_equal(f32(out, want.shape).view(np.uint32), got.view(np.uint32))
+print("recorded ok")
+"""
+    res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100, cwd=ROOT)
+    assert res.returncode == 0 and "recorded ok" in res.stdout, res.stderr[-2000:]
