@@ -367,8 +367,10 @@ int tm_hip_rope_store_f32(tm_hip_ctx *ctx, const tm_hip_rope *rope, const tm_hip
  *     slopes: x -= slopes[h] * |p - j|
  * out = sum_j softmax(x)_j * v_j. Where nothing is visible, or every visible
  * score is -infinity, out is zero. What is cached at positions a query does not
- * see has no influence on it, infinities and NaN included (an infinite key or value
- * that it does see may make its result NaN). Scores, softmax
+ * see has no influence on it, infinities and NaN included. Of what it does see, a
+ * score of -infinity takes its position out, whichever kernel a call gets; a score of
+ * infinity makes the result NaN, and so may an infinite value, or an infinite key
+ * over F16 pages at a channel where q is below 2^-37 of its row's largest. Scores, softmax
  * statistics and sums are f32; over F16 pages q and the softmax weights enter the
  * matrix products as the sum of two f16 numbers (22 bits), not rounded to one.
  * slopes (f32 [q_heads]), first (u32, one per query row: where its document

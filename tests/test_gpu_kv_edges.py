@@ -12,7 +12,7 @@ import kvutil as K
 from tuckmill_amd import hip as H
 
 from q8util import require_gpu, upload_new
-from test_gpu_kv import f32, run_decode, run_prefill, want_decode
+from test_gpu_kv import f32, prefill_case, run_decode, run_prefill, want_decode, want_prefill
 from test_gpu_kv_many import many
 
 pytestmark = pytest.mark.gpu
@@ -60,6 +60,36 @@ def test_decode_one_infinite_score_takes_its_position_out(ctx, type_id, d):
     want, tol = want_decode(clean, q, heads, 0.125, seen=seen)
     near(got, want, tol)
     assert not got[2].any()  # the only position it had
+
+
+@pytest.mark.parametrize("type_id,heads,d,news,lens", [
+    (K.F16, 3, 64, [5, 2], [100, 40]), (K.F16, 2, 256, [20, 1], [100, 40]), (K.F32, 3, 64, [5, 2], [100, 40]),
+    (K.F32, 2, 256, [20, 1], [100, 40]), (K.F16, 64, 64, [130, 6], [150, 40]), (K.F16, 64, 128, [130, 6], [150, 40]),
+    (K.F16, 64, 256, [130, 6], [150, 40]), (K.F16, 64, 72, [130, 6], [150, 40]), (K.F16, 40, 64, [300, 40], [3000, 1100]),
+    (K.F16, 16, 128, [600, 40], [1500, 1100])])
+@pytest.mark.parametrize("cap,slopes", [(0.0, False), (5.0, False), (0.0, True)])
+def test_rows_of_one_infinite_score_are_the_same_however_many_there_are(ctx, type_id, heads, d, news, lens, cap, slopes):
+    """As above for ragged rows, few (as the kernel of single tokens takes them) and many (in tiles, and
+    over positions shared between workgroups): which kernel runs does not show. Under a cap such a score is
+    minus the cap."""
+    rng = np.random.default_rng(55)
+    out_of = [n - 30 for n in lens]
+    paged = K.Paged(rng, type_id, 32, heads, d, lens)
+    clean = K.Paged(rng, type_id, 32, heads, d, lens)
+    clean.values, clean.keys = paged.values, [k.copy() for k in paged.keys]
+    seen = [np.ones(n, bool) for n in lens]
+    for s, j in enumerate(out_of):
+        for p, low in ((paged, -np.inf), (clean, -6e4)):
+            p.keys[s][j, :, 3] = low
+            p.put(s, j)
+        seen[s][j] = cap > 0  # (-6e4 is as far below the cap)
+    starts, _, _ = prefill_case(rng, news, lens)
+    q = np.abs(rng.standard_normal((sum(news), heads * d))).astype(np.float32) + np.float32(0.1)
+    sl = (2.0 ** -(1 + np.arange(heads) / 8)).astype(np.float32) if slopes else None
+    attn = H.Attention(0.125, cap, slopes=upload_new(ctx, sl) if slopes else None)
+    got = run_prefill(ctx, paged, q, heads, attn, starts)
+    want, tol = want_prefill(clean, q, heads, starts, news, 0.125, softcap=cap, slopes=sl, seen=seen)
+    near(got, want, tol)
 
 
 # ---- huge queries --------------------------------------------------------------------------------

@@ -492,10 +492,14 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
     }
 
     // channel of value v of tile t: 32 t + 8 (v / 4) + 4 h + v % 4
+    float *out = a.out + (size_t)row * a.out_stride + (size_t)head * hd;
+    // (shared positions: by way of LDS, so that a wave's stores lie side by side; units swapped as in a stage)
+    float *all = (float *)lds;
+    static_assert(4 * S::BYTES == 128 * D * 4, "results");
+    auto unit_of = [&](uint32_t unit) { return (f32x4 *)(all + (wave * 32u + c) * D + (unit ^ (c & 15u)) * 4u); };
     if (parts == 1u) {
         if (live) {
             const float by = l == 0.0f ? 0.0f : 1.0f / l;
-            float *out = a.out + (size_t)row * a.out_stride + (size_t)head * hd;
 #pragma unroll
             for (int t = 0; t < S::DT; ++t) {
 #pragma unroll
@@ -507,6 +511,84 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
                 }
             }
         }
+    } else {
+#pragma unroll
+        for (int t = 0; t < S::DT; ++t) {
+#pragma unroll
+            for (int v = 0; v < 16; v += 4) {
+                *unit_of(8u * t + v / 2u + h) = f32x4{o[t][v], o[t][v + 1], o[t][v + 2], o[t][v + 3]};
+            }
+        }
+    }
+    // A score may have come out as NaN that is an infinity: the two parts of q share a sum, and an
+    // infinite key meets each with a sign of its own, or as a zero. Rows of such are gone through again
+    // in f32, with their results in LDS, as far as they do not turn out NaN after all. Rare, and slow.
+    const bool again = live && l != l;
+    if (__any(again)) {
+        // (what this needs is taken again from the lane's number and the kernel's arguments, or it
+        // would stay in registers over the loop)
+        uint32_t lane_here = lane;
+        auto kernel_args = (const __attribute__((address_space(4))) PrefillArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+v"(lane_here), "+s"(kernel_args));
+        const AttnArgs a = *(const AttnArgs *)&kernel_args->a;
+        const uint32_t c = lane_here & 31u, h = lane_here >> 5, r = again ? tile * 128u + wave * 32u + c : 0u;
+        const uint32_t query = r / a.group, head = kvh * a.group + r % a.group;
+        const float *q_row = a.q + (size_t)(row0 + query) * a.q_stride + (size_t)head * hd;
+        float *out = a.out + (size_t)(row0 + query) * a.out_stride + (size_t)head * hd;
+        const int p = len - n + (int)query;
+        const float slope = a.slopes != nullptr ? a.slopes[head] * LOG2E : 0.0f;
+        int lo, hi;
+        visible(a, len, seq, row0 + query, p, lo, hi);
+        auto unit_of = [&](uint32_t unit) { return (f32x4 *)(all + (wave * 32u + c) * D + (unit ^ (c & 15u)) * 4u); };
+        const float by = score_factor(a.scale, a.softcap);
+        l = again ? 0.0f : l;
+        top = again ? -3.402823466e38f : top;
+        for (uint32_t d = 4u * h; again && d < hd; d += 8u) {
+            *unit_of(d / 4u) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        const int last = min((int)(start + s_end * S::N), any_hi);
+        for (int at = max((int)(start + s_begin * S::N), any_lo); at < last && __any(again && l == l); ++at) {
+            const uint32_t page = table[min((uint32_t)at >> shift, last_entry)];
+            const size_t place = ((size_t)(page < a.cache.pages ? page : 0u) * a.cache.kv_heads + kvh) * page_elements;
+            const T *k = (const T *)a.cache.k + place + ((uint32_t)at & in_page) * hd;
+            const T *v = (const T *)a.cache.v + place + ((uint32_t)at & in_page);
+            float x[1] = {0.0f};
+            for (uint32_t d = 4u * h; d < hd; d += 8u) {
+#pragma unroll
+                for (uint32_t j = 0; j < 4u; ++j) {
+                    x[0] = fmaf(q_row[d + j], (float)k[d + j], x[0]);
+                }
+            }
+            x[0] = (x[0] + __shfl_xor(x[0], 32)) * by;
+            if (a.softcap > 0.0f) {
+                cap_of(x, cap_log2);
+            }
+            if (a.slopes != nullptr) {
+                x[0] = fmaf(-slope, fabsf((float)(at - p)), x[0]);
+            }
+            if (again && at >= lo && at < hi && page < a.cache.pages) {
+                const float most = fmaxf(top, x[0]), keep = exp2_of(top - most), w = exp2_of(x[0] - most);
+                top = most;
+                l = fmaf(l, keep, w);
+                for (uint32_t d = 4u * h; d < hd; d += 8u) {
+                    f32x4 y = *unit_of(d / 4u);
+#pragma unroll
+                    for (uint32_t j = 0; j < 4u; ++j) {
+                        y[j] = fmaf(y[j], keep, w * (float)v[(d + j) << shift]);
+                    }
+                    *unit_of(d / 4u) = y;
+                }
+            }
+        }
+        for (uint32_t d = 4u * h; parts == 1u && again && d < hd; d += 8u) {
+            const f32x4 y = *unit_of(d / 4u);
+#pragma unroll
+            for (uint32_t j = 0; j < 4u; ++j) {
+                out[d + j] = l == 0.0f ? 0.0f : y[j] / l;
+            }
+        }
+    }
+    if (parts == 1u) {
         return;
     }
     // Shared positions: the parts go to memory, and the last workgroup of the tile to
@@ -515,17 +597,6 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
     const size_t slot = (size_t)want * a.cache.kv_heads + kvh;
     const float *first = args.partials + slot * args.splits * part_floats;
     const uint32_t here = min(128u, rows - tile * 128u), pairs = hd / 2u;
-    // (by way of LDS, so that a wave's stores lie side by side; units swapped as in a stage)
-    float *all = (float *)lds;
-    static_assert(4 * S::BYTES == 128 * D * 4, "results");
-#pragma unroll
-    for (int t = 0; t < S::DT; ++t) {
-#pragma unroll
-        for (int v = 0; v < 16; v += 4) {
-            const uint32_t at = wave * 32u + c, unit = 8u * t + v / 2u + h;
-            *(f32x4 *)(all + at * D + (unit ^ (c & 15u)) * 4u) = f32x4{o[t][v], o[t][v + 1], o[t][v + 2], o[t][v + 3]};
-        }
-    }
     __syncthreads();
     {
         float *to = (float *)first + split * part_floats;
@@ -601,10 +672,10 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
                 y1 += f * u[1];
             }
             const uint32_t rr = tile * 128u + at;
-            float *out = a.out + (size_t)(row0 + rr / a.group) * a.out_stride + (size_t)(kvh * a.group + rr % a.group) * hd + d;
+            float *to = a.out + (size_t)(row0 + rr / a.group) * a.out_stride + (size_t)(kvh * a.group + rr % a.group) * hd + d;
             const bool none = factor[0][at] < 0.0f; // (whatever the values: a part of no weight may hold NaN)
-            out[0] = none ? 0.0f : y0;
-            out[1] = none ? 0.0f : y1;
+            to[0] = none ? 0.0f : y0;
+            to[1] = none ? 0.0f : y1;
         }
     }
 }
