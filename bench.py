@@ -22,6 +22,11 @@ resident in HBM before the timed region. One JSON line is printed:
                           activations (config 4)
   cpu_baseline  the scalar CPU oracle timed on this host (reported only),
              with a bounded sample per configuration under per_config
+
+The line is kept below LINE_BYTES (whoever keeps only the end of a program's
+output still has all of it): numbers besides the headline's have five digits,
+and of the other configurations it has the figures, not their descriptions.
+--report FILE writes everything.
 """
 from __future__ import annotations
 
@@ -53,6 +58,54 @@ DECODE_STEP_TRAFFIC_SOURCE = ("constant from profiles/gemv_list_kernel__decode_s
                               "(rocprofv3 --pmc FETCH_SIZE / WRITE_SIZE runs of `bench.py --workload "
                               "traffic` on q8::gemv_list_kernel<1, 8, 1, true, 0, 224, false, false>); not "
                               "measured in this run")
+
+
+LINE_BYTES = 7400
+# Of the other configurations' entries the line keeps these.
+LEG_FIGURES = ("bound", "us", "achieved", "unit", "frac", "tflops_f32_equivalent", "us_per_layer",
+               "max_norm_err_vs_cpu")
+POINT_COLUMNS = ("M", "path", "us", "frac_hbm", "tflops", "frac_mfma", "max_norm_err_vs_cpu")
+
+
+def five_digits(x):
+    if isinstance(x, float):
+        return float(f"{x:.5g}")
+    if isinstance(x, dict):
+        return {k: five_digits(v) for k, v in x.items()}
+    return [five_digits(v) for v in x] if isinstance(x, (list, tuple)) else x
+
+
+def leg_figures(leg):
+    """A configuration's entry: its figures, those of the entries in it, and its points as rows."""
+    out = {}
+    for k, v in leg.items():
+        if k == "points":
+            out["points"] = [list(POINT_COLUMNS)] + [[p.get(c) for c in POINT_COLUMNS] for p in v]
+        elif isinstance(v, dict):
+            out[k] = leg_figures(v)
+        elif k in LEG_FIGURES:
+            out[k] = v
+    return {k: v for k, v in out.items() if v != {}}
+
+
+def result_line(report: dict) -> str:
+    """The report as the one line, below LINE_BYTES whatever its legs hold."""
+    legs = [k for k in ("gemm_m512", "gemma", "sweep_2b") if k in report["roofline"]]
+    line = five_digits({k: v for k, v in report.items() if k not in ("roofline", "cpu_baseline")})
+    line.update({k: report[k] for k in ("value", "ms_per_step") if k in report})
+    line["roofline"] = five_digits({k: leg_figures(v) if k in legs else v for k, v in report["roofline"].items()})
+    if "cpu_baseline" in report:
+        line["cpu_baseline"] = five_digits(report["cpu_baseline"])
+        line["cpu_baseline"]["per_config"] = {k: {n: v for n, v in c.items() if n != "sample"} for k, c in
+                                              line["cpu_baseline"].get("per_config", {}).items()}
+    drop = [("cpu_baseline", "per_config")] + [("roofline", k) for k in reversed(legs)]
+    text = json.dumps(line, separators=(",", ":"))
+    while len(text) > LINE_BYTES and drop:
+        where, k = drop.pop(0)
+        if k in line.get(where, {}):
+            line[where][k] = "left out of the line (--report)"
+        text = json.dumps(line, separators=(",", ":"))
+    return text
 
 
 class tmh_product(ctypes.Structure):
@@ -1056,6 +1109,8 @@ def main():
     ap.add_argument("--warmup", type=int, default=300)
     ap.add_argument("--cpu-seconds", type=float, default=12.0,
                     help="budget of the CPU-baseline leg (0 skips it)")
+    ap.add_argument("--report", metavar="FILE",
+                    help="decode workload: write everything that the line is made from to FILE")
     ap.add_argument("--no-gemm", action="store_true",
                     help="decode workload: leave out roofline.gemm_m512 (BASELINE config 2)")
     ap.add_argument("--no-configs", action="store_true",
@@ -1180,7 +1235,10 @@ def main():
         line["roofline"]["sweep_2b"], per_config["config4_sweep_2b"] = bench_sweep(
             host, ctx, max(40, args.steps // 4), 0, cpu=cpu, batches=SWEEP_HEADLINE_M + (16, 32, 128))
     ctx.close()
-    print(json.dumps(line), flush=True)
+    if args.report:
+        with open(args.report, "w") as f:
+            json.dump(line, f, indent=1)
+    print(result_line(line), flush=True)
 
 
 if __name__ == "__main__":
