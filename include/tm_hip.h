@@ -372,7 +372,9 @@ int tm_hip_rope_store_f32(tm_hip_ctx *ctx, const tm_hip_rope *rope, const tm_hip
  * infinity makes the result NaN, and so may an infinite value, or an infinite key
  * over F16 pages at a channel where q is below 2^-37 of its row's largest. Scores, softmax
  * statistics and sums are f32; over F16 pages q and the softmax weights enter the
- * matrix products as the sum of two f16 numbers (22 bits), not rounded to one.
+ * matrix products as the sum of two f16 numbers, not rounded to one: 22 bits of the
+ * row's largest magnitude for q, and 22 bits of a weight or 2^-31 of the row's
+ * largest, whichever is more, for the weights.
  * slopes (f32 [q_heads]), first (u32, one per query row: where its document
  * begins) and prefix (u32, one per sequence: leading positions that every query
  * of the sequence sees) may be NULL. */
@@ -390,7 +392,9 @@ typedef struct tm_hip_attn {
  * 2^30). Rows of q and out are q_heads * head_dim values from q_off, out_off,
  * strides of 0 mean packed. q_heads is a multiple of kv_heads. A long sequence is
  * split over workgroups and joined in the same launch, in the order of
- * positions: the same call gives the same bits. */
+ * positions: the same call gives the same bits. A call of more than 512 sequences
+ * does not split: each is one workgroup's for every eight (F32 pages: sixteen) query
+ * heads of a key-value head, so a long one among them is better called apart. */
 int tm_hip_attn_decode_f32(tm_hip_ctx *ctx, const tm_hip_attn *attn, const tm_hip_kv_cache *cache,
                            tm_hip_buffer *q, tm_hip_buffer *table, tm_hip_buffer *lens,
                            tm_hip_buffer *out, uint32_t seqs, uint32_t q_heads,

@@ -1,4 +1,4 @@
-// Attention of one query per sequence over the paged cache.
+// Attention over the paged cache of one query per sequence, of few ragged rows, and of all rows over f32 pages.
 #pragma once
 
 #include "kv_common.hpp"
@@ -223,7 +223,9 @@ template <int N> __device__ __forceinline__ void wait_fetches() {
 // Stages of a wave in LDS: two, where one query per sequence waits for memory (48 ragged sequences
 // of 128 channels 155 us, with one 162), or one for keys and values in turn, which leaves room for
 // more workgroups, where several rows share them (2000 f32 rows of 128 channels 115 us, with two
-// 139) or a stage is large (1500 of 256 channels 69, with two 95).
+// 139; 1500 of 256 channels 69, with two 95) or a stage is large: one query per sequence of 256 f32
+// channels takes as long with two (16 sequences with a window 30.3 and 30.3, 64 of 2000 67.2 and 67.7, one
+// of 600 12.8 and 13.0, one of 100000 101 and 97) until a CU has several workgroups (200 of 700 76 and 85).
 template <typename T, int D, bool RAGGED> struct DecodeShape {
     static constexpr int RING = RAGGED || D > 128 ? 1 : 2;
     static constexpr int COLS = sizeof(T) == 2 ? 8 : 16, PITCH = D + 4;
@@ -246,13 +248,15 @@ template <typename T, int D, bool RAGGED> struct DecodeShape {
 // tile, pages and places move the scalar base.
 // The softmax runs over one pass: weights are 2^(x - m + 6) with a reference m
 // per row that follows the maximum only when that has moved by more than 8 (so weights
-// stay below 2^14, exact in two f16 parts, and most tiles need no exchange between
-// lanes); l and o are their f32 sums. The waves join in LDS, the workgroups of a
+// stay below 2^14, and most tiles need no exchange between lanes); two f16 parts hold 22 bits
+// of a weight, or where it is below 2^-3 (the row's largest is 2^6 and more) 2^-25; l and o are
+// f32 sums. The waves join in LDS, the workgroups of a
 // unit through memory: the last to arrive adds the parts up in the order of
 // their positions.
 // Bound by memory where queries are few: one sequence of 131071 tokens, 8 heads of 128
-// channels in f16, 100 us = 5.4 TB/s; 777 tokens 9 us, of which the launch is most. Short calls
-// are bound by the way through the code, every line of which is fetched once: loads of q in
+// channels in f16, 100 us = 5.4 TB/s. Short calls (777 tokens 9 us, where a kernel that does next to nothing
+// takes 3) are bound by a chain of waits (lengths, share, table, first pages, parts, join) and the
+// way through the code, every line of which is fetched once: loads of q in
 // wide pieces and a rolled join (20 KB of code for 30) took 16 sequences in f32 from 57 to 30 us.
 // Bound by the f32 matrix cores where f32 rows are many: two sequences of 2000 rows, 16 heads of 128
 // channels, 347 us.

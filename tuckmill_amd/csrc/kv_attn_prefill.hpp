@@ -121,9 +121,10 @@ template <int D, bool FULL> struct Rows {
 // In LDS the 16-byte units of a row are swapped by exclusive or with the row's number,
 // which spreads a column of units over the banks.
 // Bound by the matrix cores where rows are many: a prompt of 8192, 32 heads of 128 channels,
-// 950 us = 580 TFLOP/s (1160 with both parts of q and of the weights counted); 4001 rows of packed
-// documents of 64 channels with bias and cap 54 us, bound by what happens to each score and, at six
-// steps a workgroup, by how each begins and ends.
+// 960 us = 575 TFLOP/s (1150 with both parts of q and of the weights counted). 4001 rows of packed
+// documents of 64 channels with bias and cap 55 us: vector instructions, 18 a score, keep a SIMD busy for
+// 42% of it; the rest is that tiles have 1 to 13 steps, six on average, and are all there at once, so
+// that some CUs end early, and how each begins and ends.
 template <int D, bool FULL, int WAVES_PER_SIMD>
 __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(PrefillArgs args) {
     typedef _Float16 T;

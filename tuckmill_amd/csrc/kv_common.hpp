@@ -22,8 +22,8 @@ __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2
 
 // x = cap * tanh(x) for a lane's scores (x = score / cap; cap in units of log2 e), tanh
 // to a few half steps relative to its value: its series below 1/2 (the first term left
-// out is 5e-9 of it there) and below 1/4 (2e-9, five terms); above, (1 - t) / (1 + t) with
-// t = exp(-2 |x|). The ways are chosen for the wave: scores are mostly well below their cap.
+// out is 9.7e-9 of tanh there, a sixth of a half step) and below 1/4 (8.6e-9, five terms);
+// above, (1 - t) / (1 + t) with t = exp(-2 |x|). The ways are chosen for the wave: scores are mostly well below their cap.
 template <int N> __device__ __forceinline__ void cap_of(float (&x)[N], float cap) {
     float most = 0.0f;
 #pragma unroll

@@ -17,7 +17,11 @@ inline uint32_t decode_cols(uint32_t type_id) { return type_id == 1u ? 8u : 16u;
 constexpr uint32_t DECODE_SHARES = 256;
 constexpr uint64_t DECODE_MAX_GRID = 1u << 23; // (a dimension of a grid is below 2^32 threads)
 constexpr uint32_t DECODE_WAVES = 4; // of a workgroup
-constexpr uint32_t DECODE_MAX_SEQS = 512; // whose work is shared out (every workgroup goes through all of them)
+// Sequences whose work is shared out. Every workgroup then goes through all of them, which their number
+// makes dearer and a long one among them makes worth it. (In us, 16 heads of 128 channels on 8, f16, shared and
+// not: 513 sequences of 200 135 and 106, one of them of 100000 189 and 1200; 1024 308 and 195, with one 352 and
+// 1240; 2048 882 and 362, with one 847 and 1326.)
+constexpr uint32_t DECODE_MAX_SEQS = 512;
 
 struct AttnPlan {
     bool tiled = false;      // ragged rows: with the prefill kernel (else the decode kernel's)
@@ -64,7 +68,8 @@ constexpr uint64_t PREFILL_MAX_GROUPS = 1u << 23;
 // to 64, 2000 and 16000 cached positions: of 128 channels at 1032 units 20, 39, 127 and 21, 53, 92, at
 // 2056 38, 66, 281 and 30, 57, 153; of 64 channels at 776 11, 15, 33 and 14, 22, 36, at 1544 21, 35, 88
 // and 20, 32, 58; of 256 channels at 516 26, 43, 152 and 52, 105, 190, at 1028 58, 92, 490 and 91, 120,
-// 333.) Pages of f32 it takes always: their products go at
+// 333: near the limit long caches would be better off with the prefill kernel, short ones not, and which they
+// are only the device knows; here there is the room in the table.) Pages of f32 it takes always: their products go at
 // a sixteenth of f16's rate, and its waves of 16 rows fill the card better than tiles of
 // 128 did (1500 rows of 256 channels 69 and 138, 4000 926 and 1216, 4000 of 128 347 and 509).
 constexpr uint64_t DECODE_MAX_UNITS = 1056;
@@ -101,7 +106,8 @@ inline AttnPlan prefill_plan(uint32_t type_id, uint32_t seqs, uint32_t tokens, u
 }
 
 // Ids of a workgroup that adjusts logits: large tiles where they still give every CU one. (In us, large
-// and small, rows of 151936: one 7.9 and 6.1, 16 8.0 and 6.2, 64 with histories of 4096 20 and 30.)
+// and small, rows of 151936: one 7.8 and 7.8, 16 7.9 and 7.6, 64 with histories of 4096 20 and 30; the shortest
+// of a call's times 6.6 and 6.4, 7.2 and 7.0.)
 constexpr uint32_t LOGITS_LARGE = 8192, LOGITS_SMALL = 1024, LOGITS_MIN_GROUPS = 256;
 
 } // namespace kv

@@ -63,12 +63,6 @@ void alloc_release(Alloc *a) {
     }
 }
 
-// An operation recorded into an open group holds a reference on every
-// allocation it names from the moment it is recorded (the reference's group
-// leases its buffers at encode time, native/metal/tm_metal.m:673, :707-739): a
-// handle may be freed before end_group and the memory lives on. The references
-// are dropped once the commit (or the recorded step) has taken its own, or when
-// the group is aborted.
 // Every allocation an operation names, those of its KvParams included.
 template <typename F> void each_alloc(const Op &op, F f) {
     for (int i = 0; i < op.n_alloc; ++i) {
@@ -85,6 +79,12 @@ template <typename F> void each_alloc(const Op &op, F f) {
     }
 }
 
+// An operation recorded into an open group holds a reference on every
+// allocation it names from the moment it is recorded (the reference's group
+// leases its buffers at encode time, native/metal/tm_metal.m:673, :707-739): a
+// handle may be freed before end_group and the memory lives on. The references
+// are dropped once the commit (or the recorded step) has taken its own, or when
+// the group is aborted.
 void ops_hold(const Op &op) {
     each_alloc(op, [](Alloc *a) { a->refs.fetch_add(1, std::memory_order_relaxed); });
 }
