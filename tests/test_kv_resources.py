@@ -1,5 +1,6 @@
-"""Registers of the attention kernels, checked at compile time (no GPU): none of the forms that a short
-call waits for may keep registers in scratch memory, and two workgroups must fit a CU."""
+"""Registers of the attention kernels, checked at compile time (no GPU): of the forms that a short call
+waits for, those of single tokens and those of few rows of up to 128 channels keep none in scratch memory,
+few rows of 256 channels no more than a dozen, and two workgroups fit a CU."""
 import os
 import re
 import shutil
@@ -50,3 +51,18 @@ def test_tiles_of_rows_fit_two_workgroups_per_cu(kernels):
         assert spilled == 0 and waves >= 2, registers
     for registers, spilled, waves in of(kernels, r"attn_prefill_kernelILi128E"):
         assert waves >= 2, registers
+
+
+def test_few_rows_of_256_channels_keep_all_but_a_dozen_registers(kernels):
+    for registers, spilled, waves in of(kernels, r"attn_decode_kernelI(DF16_|f)Li256ELb[01]ELb1E"):
+        assert spilled <= 12 and waves >= 2, (registers, spilled)
+
+
+def test_tiles_of_rows_of_256_channels_fit_a_cu(kernels):
+    for registers, spilled, waves in of(kernels, r"attn_prefill_kernelILi256E"):
+        assert spilled <= 24 and waves >= 1, (registers, spilled)
+
+
+def test_tiles_of_rows_of_64_channels_fit_three_workgroups_per_cu(kernels):
+    for registers, spilled, waves in of(kernels, r"attn_prefill_kernelILi64E"):
+        assert spilled == 0 and waves >= 3, registers
