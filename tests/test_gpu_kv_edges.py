@@ -92,6 +92,39 @@ def test_rows_of_one_infinite_score_are_the_same_however_many_there_are(ctx, typ
     near(got, want, tol)
 
 
+@pytest.mark.parametrize("every", [64, 700])
+def test_rows_of_many_infinite_scores_beside_rows_that_are_nan(ctx, every):
+    """Few and many positions to take out (and those of them in the first pages and the last), a query that
+    is NaN, one that is infinite, and a key that is NaN to the rows that see it."""
+    rng = np.random.default_rng(56)
+    heads, d, rows, n = 64, 64, 600, 3000
+    assert many(rows, 1, heads, heads)
+    paged = K.Paged(rng, K.F16, 32, heads, d, [n])
+    clean = K.Paged(rng, K.F16, 32, heads, d, [n])
+    seen = np.ones(n, bool)
+    seen[5::every] = False
+    seen[n - rows + 20] = False  # a position that only some rows see
+    clean.keys = [paged.keys[0].copy()]
+    clean.values = paged.values
+    paged.keys[0][~seen, :, 3] = -np.inf
+    paged.keys[0][n - 40, :, 7] = np.nan
+    for j in range(n):
+        paged.put(0, j)
+    q = np.abs(rng.standard_normal((rows, heads * d))).astype(np.float32) + np.float32(0.1)
+    q[33] = np.nan
+    q[77, 3::d] = np.inf
+    got = run_prefill(ctx, paged, q, heads, H.Attention(0.125), np.array([0, rows]))
+    p = np.arange(n - rows, n)
+    fine = (p < n - 40) & ~np.isin(np.arange(rows), [33, 77])
+    lo, hi = K.bounds(p, n)
+    for r0 in range(0, rows, 37):  # (some of the rows: the reference is slow)
+        r = np.array([r0, min(r0 + 1, rows - 1)])
+        want, tol = K.attention(q[r].reshape(len(r), heads, d), clean.keys[0], clean.values[0], p[r], lo[r], hi[r], 0.125, seen=seen)
+        near(got[r][fine[r]], want[fine[r]], tol[fine[r]], f"row {r0}")
+    assert np.isnan(got[33]).all() and np.isnan(got[77]).all() and np.isnan(got[p >= n - 40]).all()
+    assert not np.isnan(got[fine]).any()
+
+
 # ---- huge queries --------------------------------------------------------------------------------
 
 def check_decided(got, scores, error, values, margin):

@@ -27,6 +27,8 @@ template <int D> struct PrefillShape {
     static constexpr int SWIZZLE = UK < 16 ? UK - 1 : 15;
 };
 
+constexpr uint32_t ASIDE = 32; // steps that a wave puts aside; where there are more it goes through all again
+
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -133,7 +135,7 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
     typedef typename R::Unit Unit;
     extern __shared__ __align__(1024) uint8_t lds[]; // two stages of keys and values
     __shared__ int range[4][2];
-    __shared__ uint32_t arrived, cleaned;
+    __shared__ uint32_t arrived, cleaned, aside[4][ASIDE];
     __shared__ float factor[PREFILL_MAX_SPLITS][128];
     const AttnArgs &a = args.a;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -255,6 +257,7 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
         }
     }
     float top = -3.402823466e38f, l = 0.0f;
+    uint32_t asides = 0; // steps put aside
     for (uint32_t step = s_begin; step < s_end; ++step) {
 #pragma unroll
         for (int i = 0; i < PAGES; ++i) {
@@ -362,15 +365,47 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
                 }
             }
         }
-        float most = x[0][0];
+        float most = x[0][0]; // or NaN, which any of them hands on
 #pragma unroll
         for (int b = 0; b < S::SUB; ++b) {
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
-                most = fmaxf(most, x[b][v]);
+                most = __builtin_elementwise_maximum(most, x[b][v]);
             }
         }
-        if (__any(most > top + 14.0f)) {
+        if (__any(!(most <= top + 14.0f))) {
+            if (__any(most != most)) {
+                // A score may be NaN that should be an infinity: the two parts of q share a sum, and an infinite
+                // key meets each with a sign of its own, or as a zero. The step is put aside for the wave, to
+                // be gone through in f32 after the loop, unless only rows have it that are NaN anyway: of a q
+                // that is not finite, or a score of infinity.
+                Unit odd = {};
+#pragma unroll
+                for (int i = 0; i < S::KS; ++i) {
+                    odd = __builtin_elementwise_fma(q.hi[i], Unit{}, odd);
+                }
+                bool lost = l != l || !(top < INFINITY);
+#pragma unroll
+                for (int j = 0; j < S::E; ++j) {
+                    lost = lost || odd[j] != (T)0.0f;
+                }
+                lost = __shfl_xor((int)lost, 32) != 0 || lost;
+                if (__any(most != most && !lost)) {
+                    if (lane == 0u) {
+                        aside[wave][asides % ASIDE] = step;
+                    }
+                    ++asides;
+                    l = lost ? NAN : l;
+                    most = -INFINITY;
+#pragma unroll
+                    for (int b = 0; b < S::SUB; ++b) {
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) {
+                            x[b][v] = -INFINITY;
+                        }
+                    }
+                }
+            }
             most = fmaxf(most, __shfl_xor(most, 32));
             most = fmaxf(most - 6.0f, top);
             const float keep = exp2_of(top - most);
@@ -498,7 +533,7 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
     float *all = (float *)lds;
     static_assert(4 * S::BYTES == 128 * D * 4, "results");
     auto unit_of = [&](uint32_t unit) { return (f32x4 *)(all + (wave * 32u + c) * D + (unit ^ (c & 15u)) * 4u); };
-    if (parts == 1u) {
+    if (parts == 1u && asides == 0u) {
         if (live) {
             const float by = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -521,19 +556,17 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
             }
         }
     }
-    // A score may have come out as NaN that is an infinity: the two parts of q share a sum, and an
-    // infinite key meets each with a sign of its own, or as a zero. Rows of such are gone through again
-    // in f32, with their results in LDS, as far as they do not turn out NaN after all. Rare, and slow.
-    const bool again = live && l != l;
-    if (__any(again)) {
+    // The steps put aside, or, of more than there is room for, all: in f32, with the rows' results in LDS. Rare, and slow.
+    if (asides != 0u) {
         // (what this needs is taken again from the lane's number and the kernel's arguments, or it
         // would stay in registers over the loop)
         uint32_t lane_here = lane;
         auto kernel_args = (const __attribute__((address_space(4))) PrefillArgs *)__builtin_amdgcn_kernarg_segment_ptr();
         asm volatile("" : "+v"(lane_here), "+s"(kernel_args));
         const AttnArgs a = *(const AttnArgs *)&kernel_args->a;
-        const uint32_t c = lane_here & 31u, h = lane_here >> 5, r = again ? tile * 128u + wave * 32u + c : 0u;
-        const uint32_t query = r / a.group, head = kvh * a.group + r % a.group;
+        const uint32_t c = lane_here & 31u, h = lane_here >> 5, r = tile * 128u + wave * 32u + c;
+        const bool live = r < rows, all_steps = asides > ASIDE;
+        const uint32_t query = live ? r / a.group : 0u, head = kvh * a.group + (live ? r % a.group : 0u);
         const float *q_row = a.q + (size_t)(row0 + query) * a.q_stride + (size_t)head * hd;
         float *out = a.out + (size_t)(row0 + query) * a.out_stride + (size_t)head * hd;
         const int p = len - n + (int)query;
@@ -542,46 +575,53 @@ __global__ __launch_bounds__(256, WAVES_PER_SIMD) void attn_prefill_kernel(Prefi
         visible(a, len, seq, row0 + query, p, lo, hi);
         auto unit_of = [&](uint32_t unit) { return (f32x4 *)(all + (wave * 32u + c) * D + (unit ^ (c & 15u)) * 4u); };
         const float by = score_factor(a.scale, a.softcap);
-        l = again ? 0.0f : l;
-        top = again ? -3.402823466e38f : top;
-        for (uint32_t d = 4u * h; again && d < hd; d += 8u) {
-            *unit_of(d / 4u) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
-        const int last = min((int)(start + s_end * S::N), any_hi);
-        for (int at = max((int)(start + s_begin * S::N), any_lo); at < last && __any(again && l == l); ++at) {
-            const uint32_t page = table[min((uint32_t)at >> shift, last_entry)];
-            const size_t place = ((size_t)(page < a.cache.pages ? page : 0u) * a.cache.kv_heads + kvh) * page_elements;
-            const T *k = (const T *)a.cache.k + place + ((uint32_t)at & in_page) * hd;
-            const T *v = (const T *)a.cache.v + place + ((uint32_t)at & in_page);
-            float x[1] = {0.0f};
+        if (all_steps) {
+            l = l == l ? 0.0f : l;
+            top = -3.402823466e38f;
             for (uint32_t d = 4u * h; d < hd; d += 8u) {
-#pragma unroll
-                for (uint32_t j = 0; j < 4u; ++j) {
-                    x[0] = fmaf(q_row[d + j], (float)k[d + j], x[0]);
-                }
+                *unit_of(d / 4u) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             }
-            x[0] = (x[0] + __shfl_xor(x[0], 32)) * by;
-            if (a.softcap > 0.0f) {
-                cap_of(x, cap_log2);
-            }
-            if (a.slopes != nullptr) {
-                x[0] = fmaf(-slope, fabsf((float)(at - p)), x[0]);
-            }
-            if (again && at >= lo && at < hi && page < a.cache.pages) {
-                const float most = fmaxf(top, x[0]), keep = exp2_of(top - most), w = exp2_of(x[0] - most);
-                top = most;
-                l = fmaf(l, keep, w);
+        }
+        const uint32_t some = all_steps ? s_end - s_begin : asides;
+        for (uint32_t i = 0; i < some; ++i) {
+            const int base = (int)(start + (all_steps ? s_begin + i : aside[wave][i]) * S::N);
+            const int last = min(base + S::N, any_hi);
+            // (as long as there is a row that is not NaN)
+            for (int at = max(base, any_lo); at < last && __any(live && l == l); ++at) {
+                const uint32_t page = table[min((uint32_t)at >> shift, last_entry)];
+                const size_t place = ((size_t)(page < a.cache.pages ? page : 0u) * a.cache.kv_heads + kvh) * page_elements;
+                const T *k = (const T *)a.cache.k + place + ((uint32_t)at & in_page) * hd;
+                const T *v = (const T *)a.cache.v + place + ((uint32_t)at & in_page);
+                float x[1] = {0.0f};
                 for (uint32_t d = 4u * h; d < hd; d += 8u) {
-                    f32x4 y = *unit_of(d / 4u);
 #pragma unroll
                     for (uint32_t j = 0; j < 4u; ++j) {
-                        y[j] = fmaf(y[j], keep, w * (float)v[(d + j) << shift]);
+                        x[0] = fmaf(q_row[d + j], (float)k[d + j], x[0]);
                     }
-                    *unit_of(d / 4u) = y;
+                }
+                x[0] = (x[0] + __shfl_xor(x[0], 32)) * by;
+                if (a.softcap > 0.0f) {
+                    cap_of(x, cap_log2);
+                }
+                if (a.slopes != nullptr) {
+                    x[0] = fmaf(-slope, fabsf((float)(at - p)), x[0]);
+                }
+                if (live && at >= lo && at < hi && page < a.cache.pages) {
+                    const float most = fmaxf(top, x[0]), keep = exp2_of(top - most), w = exp2_of(x[0] - most);
+                    top = most;
+                    l = fmaf(l, keep, w);
+                    for (uint32_t d = 4u * h; d < hd; d += 8u) {
+                        f32x4 y = *unit_of(d / 4u);
+#pragma unroll
+                        for (uint32_t j = 0; j < 4u; ++j) {
+                            y[j] = fmaf(y[j], keep, w * (float)v[(d + j) << shift]);
+                        }
+                        *unit_of(d / 4u) = y;
+                    }
                 }
             }
         }
-        for (uint32_t d = 4u * h; parts == 1u && again && d < hd; d += 8u) {
+        for (uint32_t d = 4u * h; parts == 1u && live && d < hd; d += 8u) {
             const f32x4 y = *unit_of(d / 4u);
 #pragma unroll
             for (uint32_t j = 0; j < 4u; ++j) {
