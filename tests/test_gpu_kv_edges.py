@@ -125,6 +125,39 @@ def test_rows_of_many_infinite_scores_beside_rows_that_are_nan(ctx, every):
     assert not np.isnan(got[fine]).any()
 
 
+@pytest.mark.parametrize("d,window,prefix,docs", [(64, 0, 0, 1), (128, 100, 0, 0), (64, 40, 1, 0), (256, 0, 1, 1)])
+def test_infinite_scores_under_masks_with_shared_heads(ctx, d, window, prefix, docs):
+    """Four query heads to a key-value head, odd strides, biases and every mask: what is taken out is what
+    each row sees of it."""
+    rng = np.random.default_rng(57)
+    heads, kv_heads, news, lens = 32, 8, [270, 33], [500, 60]
+    assert many(sum(news), 2, heads, kv_heads)
+    paged = K.Paged(rng, K.F16, 16, kv_heads, d, lens)
+    clean = K.Paged(rng, K.F16, 16, kv_heads, d, lens)
+    clean.keys, clean.values = [k.copy() for k in paged.keys], paged.values
+    seen = [rng.random(n) > 0.03 for n in lens]
+    for s, n in enumerate(lens):
+        paged.keys[s][~seen[s], :, 3] = -np.inf
+        for j in range(n):
+            paged.put(s, j)
+    starts, first, pre = prefill_case(rng, news, lens, docs, prefix)
+    w = heads * d
+    q = np.abs(rng.standard_normal((sum(news), w))).astype(np.float32) + np.float32(0.1)
+    flat = np.full((sum(news), w + 3), np.nan, np.float32)
+    flat[:, :w] = q
+    sl = (2.0 ** -(1 + np.arange(heads) / 8)).astype(np.float32)
+    attn = H.Attention(0.125, 0.0, window, slopes=upload_new(ctx, sl), first=upload_new(ctx, K.u32(first)) if docs else None,
+                       prefix=upload_new(ctx, K.u32(pre)) if prefix else None)
+    out = upload_new(ctx, np.full((sum(news), w + 1), 7.0, np.float32))
+    ctx.attn_prefill(attn, paged.upload(ctx), upload_new(ctx, flat), upload_new(ctx, paged.table), upload_new(ctx, K.u32(lens)),
+                     upload_new(ctx, K.u32(starts)), out, sum(news), 2, heads, paged.stride, 0, 0, w + 3, w + 1)
+    ctx.fence()
+    got = f32(out, (sum(news), w + 1))
+    want, tol = want_prefill(clean, q, heads, starts, news, 0.125, first, window, 0.0, sl, pre, seen)
+    near(got[:, :w].reshape(want.shape), want, tol)
+    assert (got[:, w:] == 7.0).all()
+
+
 # ---- huge queries --------------------------------------------------------------------------------
 
 def check_decided(got, scores, error, values, margin):
